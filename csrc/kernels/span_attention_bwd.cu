@@ -1,0 +1,675 @@
+// Span attention backward for sm_100a (tcgen05 + TMEM + TMA), 16-bit, heads of 8 to 128 numbers.  With the scores x and weights p of the forward pass,
+// t = tanh(scale q.k / cap), and delta = sum dO O of a row:
+//
+//   dP = dO V^T,  dS = p (dP - delta) (1 - t^2),  dQ = scale dS K,  dK = scale dS^T Q,  dV = P^T dO
+//
+// Two kernels, so that every gradient is summed by one CTA in one order (no atomics: the same inputs give the same gradients) and none passes
+// through an fp32 buffer in memory: dQ by tiles of query rows, then dK and dV by tiles of keys.  Both recompute S and dP; the two extra products
+// cost what the atomics of a joint kernel would.  P and dS stay in tensor memory, where the next product takes them as its left operand.
+//
+// The first kernel also writes what the second one asks per query row: log-sum-exp, delta and the span, and per 64 rows the range of their spans,
+// by which the second kernel leaves out tiles that do not reach its keys.  dS is rounded to 16 bits before the scale, which keeps small gradients
+// of fp16 heads away from its subnormal numbers.
+#include "span_scores.cuh"
+
+namespace rb {
+
+struct SpanBwdParams {
+  int B, H, Hkv, Sq, Sk, D;
+  int tiles;                        // of the launch, along rows or keys
+  SpanScores c;
+  float scale, inv_out2;            // 1 / (cap log2 e)
+  const void *q, *o, *dout;         // o [B, Sq, H, D] contiguous
+  long long q_st[3], do_st[3];
+  const float* lse2;                // [B, H, Sq]
+  // per row, rows padded to a multiple of 64 (zeros there)
+  float *row_lse2, *row_delta;      // [B, H, sq_pad]
+  int *row_lo, *row_hi;             // [B, sq_pad]
+  int4* range;                      // [B, sq_pad / 64] {least lo, largest hi, largest lo, least hi}
+  int sq_pad;
+  void *dq, *dk, *dv;
+  long long dq_st[3], dkv_st[3];
+  int* status;
+};
+
+template <typename T>
+__device__ __forceinline__ void span_pack32(const float* f, uint32_t* w) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) w[i] = pack2<T>(f[2 * i], f[2 * i + 1]);
+}
+
+// 1 - t^2 of capped scores (log2 units), in place of which the caller goes on with the scores
+template <int N>
+__device__ __forceinline__ void span_slip(const uint32_t* s, float inv_out2, float* slip) {
+  const uint64_t k = f32x2(inv_out2, inv_out2), one = f32x2(1.f, 1.f), minus = f32x2(-1.f, -1.f);
+#pragma unroll
+  for (int i = 0; i < N; i += 2) {
+    const uint64_t t = mul_f32x2(f32x2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), k);
+    const float2 v = f32x2_get(fma_f32x2(mul_f32x2(t, minus), t, one));
+    slip[i] = v.x;
+    slip[i + 1] = v.y;
+  }
+}
+
+// ---------------------------------------------------------------- dQ
+// A CTA owns 128 query rows of a head and goes over tiles of 64 keys; two warpgroups take the tiles in turn, a thread owns a row.  Q and dO lie in
+// tensor memory: as left operands from shared memory they would take most of its port (128 bytes a clock).
+template <int HD>
+struct SpanDqCfg {
+  static constexpr int SUB = HD / 64, SUB_BYTES = 64 * 128, TILE = SUB * SUB_BYTES;
+  static constexpr int STAGES = HD == 128 ? 6 : 8;
+  static constexpr int SMEM_BYTES = STAGES * 2 * TILE + 1024 + 256;
+  static constexpr int Q_COL = 0, DO_COL = 64, DQ_COL = 128, S_COL = 256, DP_COL = 384;     // S, dP of buffer w: + 64 w
+};
+
+template <typename T, int HD, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(320, 1)
+    span_dq_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const SpanBwdParams p) {
+  using C = SpanDqCfg<HD>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::STAGES * 2 * C::TILE);       // [STAGES] {K, V}
+  uint64_t *full = bars, *empty = full + C::STAGES, *sdp_full = empty + C::STAGES, *ds_ready = sdp_full + 2, *dq_done = ds_ready + 2;
+  uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(dq_done + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_ptr + 1);
+  __shared__ int4 s_range[4];
+  __shared__ float s_delta[128];
+
+  const int warp = uniform_warp_idx(), lane = threadIdx.x & 31;
+  int idx = blockIdx.x;
+  const int q0 = (p.tiles - 1 - idx % p.tiles) * 128;                                  // causal: the longest first
+  idx /= p.tiles;
+  const int h = idx % p.H, b = idx / p.H, hkv = h / (p.H / p.Hkv);
+  const int off = p.Sk - p.Sq;
+  const int t = threadIdx.x & 127, wg = warp >> 2, row = q0 + t;
+  const bool live = row < p.Sq;
+
+  if (threadIdx.x == 0) {
+    prefetch_tensormap(&tk);
+    prefetch_tensormap(&tv);
+    for (int s = 0; s < C::STAGES; ++s) {
+      mbar_init(smem_u32(&full[s]), 1);
+      mbar_init(smem_u32(&empty[s]), 1);
+    }
+    for (int w = 0; w < 2; ++w) {
+      mbar_init(smem_u32(&sdp_full[w]), 1);
+      mbar_init(smem_u32(&ds_ready[w]), 128);
+    }
+    mbar_init(smem_u32(dq_done), 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  int2 span = make_int2(0, 0);
+  if (warp < 8) {
+    if (live) span = span_of(p.c, b, row, p.Sq, p.Sk);
+    const int4 r = span_range_warp(span, live);
+    if (warp < 4 && lane == 0) s_range[warp] = r;
+  } else if (warp == 9) {
+    tmem_alloc(smem_u32(tmem_ptr), 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_ptr;
+  const int4 half0 = span_range_join(s_range[0], s_range[1]), half1 = span_range_join(s_range[2], s_range[3]);
+  const int4 all = span_range_join(half0, half1);
+  const int j0 = all.x < all.y ? all.x / 64 : 0, n = all.x < all.y ? (all.y + 63) / 64 - j0 : 0;
+
+  const uint32_t lane_addr = tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+  float lse2 = 0.f;
+  if (warp < 8) {
+    // Q (first warpgroup) and dO (second) into tensor memory; delta on the way
+    const T* from = wg == 0 ? reinterpret_cast<const T*>(p.q) + b * p.q_st[0] + row * p.q_st[1] + h * p.q_st[2]
+                            : reinterpret_cast<const T*>(p.dout) + b * p.do_st[0] + row * p.do_st[1] + h * p.do_st[2];
+    const T* o = reinterpret_cast<const T*>(p.o) + ((static_cast<long long>(b) * p.Sq + row) * p.H + h) * p.D;
+    float delta = 0.f;
+#pragma unroll
+    for (int c = 0; c < HD / 32; ++c) {
+      uint32_t w[16];
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        uint4 v = make_uint4(0, 0, 0, 0), y = v;
+        const int d = c * 32 + g * 8;
+        if (live && d < p.D) {
+          v = *reinterpret_cast<const uint4*>(from + d);
+          if (wg == 1) y = *reinterpret_cast<const uint4*>(o + d);
+        }
+        w[g * 4] = v.x; w[g * 4 + 1] = v.y; w[g * 4 + 2] = v.z; w[g * 4 + 3] = v.w;
+        const uint32_t z[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 e = unpack2<T>(w[g * 4 + i]), f = unpack2<T>(z[i]);
+          delta = fmaf(e.x, f.x, fmaf(e.y, f.y, delta));
+        }
+      }
+      tmem_st_32x32b_x16(lane_addr + (wg == 0 ? C::Q_COL : C::DO_COL) + c * 16, w);
+    }
+    if (live && span.x < span.y) lse2 = p.lse2[(static_cast<long long>(b) * p.H + h) * p.Sq + row];
+    if (row < p.sq_pad) {
+      const long long at = (static_cast<long long>(b) * p.H + h) * p.sq_pad + row;
+      if (wg == 0) p.row_lse2[at] = lse2;
+      else p.row_delta[at] = delta;
+      if (h == 0 && wg == 0) {
+        p.row_lo[static_cast<long long>(b) * p.sq_pad + row] = span.x;
+        p.row_hi[static_cast<long long>(b) * p.sq_pad + row] = span.y;
+        if ((t & 63) == 0) {
+          int4 r = t == 0 ? half0 : half1;
+          if (row + 64 > p.Sq) r.w = 0;           // rows behind the last one see nothing: such a tile is masked
+          p.range[(static_cast<long long>(b) * p.sq_pad + row) / 64] = r;
+        }
+      }
+    }
+    if (wg == 1) s_delta[t] = delta;
+    tmem_st_wait();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+
+  if (warp == 8) {
+    // ------------------------------ TMA producer ------------------------------
+    if (lane == 0) {
+      bool ok = true;
+      int st = 0;
+      uint32_t ph = 0;
+      for (int i = 0; i < n; ++i) {
+        ok = mbar_wait(smem_u32(&empty[st]), ph ^ 1, abort_flag, p.status, RB_ERR_TIMEOUT_EMPTY);
+        if (!ok) break;
+        const uint32_t bar = smem_u32(&full[st]), dst = smem_u32(smem + st * 2 * C::TILE);
+        mbar_arrive_expect_tx(bar, 2 * C::TILE);
+#pragma unroll
+        for (int s = 0; s < C::SUB; ++s) {
+          tma_load_4d(dst + s * C::SUB_BYTES, &tk, bar, s * 64, (j0 + i) * 64, hkv, b);
+          tma_load_4d(dst + C::TILE + s * C::SUB_BYTES, &tv, bar, s * 64, (j0 + i) * 64, hkv, b);
+        }
+        if (++st == C::STAGES) { st = 0; ph ^= 1; }
+      }
+      if (!ok)
+        for (int i = 0; i < 64; ++i) __nanosleep(10000);
+    }
+  } else if (warp == 9) {
+    // ------------------------------ MMA issuer --------------------------------
+    constexpr uint32_t idesc_s = make_idesc(UmmaFormat<T>::value, 0, 0, 128, 64);
+    constexpr uint32_t idesc_q = make_idesc(UmmaFormat<T>::value, 0, 1, 128, HD);
+    bool ok = true;
+    int st_in = 0, st_out = 0;
+    uint32_t ph_in = 0;
+    auto issue = [&](int i) {            // S and dP of tile i, the next stage
+      ok = mbar_wait(smem_u32(&full[st_in]), ph_in, abort_flag, p.status, RB_ERR_TIMEOUT_FULL);
+      if (!ok) return;
+      tc_fence_after();
+      const uint32_t k = smem_u32(smem + st_in * 2 * C::TILE);
+      const uint64_t kd = make_smem_desc_sw128(k, 16, 1024), vd = make_smem_desc_sw128(k + C::TILE, 16, 1024);
+#pragma unroll
+      for (int s = 0; s < C::SUB; ++s) {
+        umma_f16_ts_w4<8, 2>(tmem_base + C::S_COL + (i & 1) * 64, tmem_base + C::Q_COL + s * 32, kd + s * (C::SUB_BYTES >> 4), idesc_s, s != 0);
+        umma_f16_ts_w4<8, 2>(tmem_base + C::DP_COL + (i & 1) * 64, tmem_base + C::DO_COL + s * 32, vd + s * (C::SUB_BYTES >> 4), idesc_s, s != 0);
+      }
+      umma_commit_w(smem_u32(&sdp_full[i & 1]));
+      if (++st_in == C::STAGES) { st_in = 0; ph_in ^= 1; }
+    };
+    for (int i = 0; i < 2 && i < n && ok; ++i) issue(i);
+    for (int i = 0; i < n && ok; ++i) {
+      ok = mbar_wait(smem_u32(&ds_ready[i & 1]), (i >> 1) & 1, abort_flag, p.status, RB_ERR_TIMEOUT_FLAG);
+      if (!ok) break;
+      tc_fence_after();
+      const uint64_t kd = make_smem_desc_sw128(smem_u32(smem + st_out * 2 * C::TILE), C::SUB_BYTES, 1024);
+      umma_f16_ts_w4<8, 128>(tmem_base + C::DQ_COL, tmem_base + C::S_COL + (i & 1) * 64, kd, idesc_q, i != 0);
+      umma_commit_w(smem_u32(&empty[st_out]));
+      if (i + 1 == n) umma_commit_w(smem_u32(dq_done));
+      if (++st_out == C::STAGES) st_out = 0;
+      if (i + 2 < n) issue(i + 2);
+    }
+  } else {
+    // ------------------------------ softmax warpgroups ------------------------
+    const float slope2 = BIAS ? p.c.slopes[h] * kLog2e : 0.f, delta = s_delta[t];
+    const uint32_t s_addr = lane_addr + C::S_COL + wg * 64, dp_addr = lane_addr + C::DP_COL + wg * 64;
+    bool ok = true;
+    for (int i = wg; i < n; i += 2) {
+      ok = mbar_wait(smem_u32(&sdp_full[wg]), (i >> 1) & 1, abort_flag, p.status, RB_ERR_TIMEOUT_TMEM_FULL);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tc_fence_after();
+      const int kv0 = (j0 + i) * 64;
+      const bool masked = kv0 < all.z || kv0 + 64 > all.w;
+      const int side = q0 + off >= kv0 + 63 ? 1 : q0 + 127 + off <= kv0 ? -1 : 0;
+      uint32_t ds[2][16];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t s[32], dp[32];
+        float g[32];
+        tmem_ld_32x32b_x32(s_addr + c * 32, s);
+        tmem_ld_32x32b_x32(dp_addr + c * 32, dp);
+        tmem_ld_wait();
+        span_scale<CAP, 32>(s, p.c);
+        if constexpr (CAP) span_slip<32>(s, p.inv_out2, g);
+        if constexpr (BIAS) span_bias<-1, 32>(s, slope2, (float)(row + off - kv0 - c * 32), side);
+#pragma unroll
+        for (int k = 0; k < 32; ++k) {
+          const float w = fast_exp2(__uint_as_float(s[k]) - lse2);
+          g[k] = CAP ? w * g[k] : w;
+        }
+#pragma unroll
+        for (int k = 0; k < 32; ++k) g[k] *= __uint_as_float(dp[k]) - delta;
+        if (masked) {
+          const uint32_t seen = span_bits(span.x - kv0 - c * 32, span.y - kv0 - c * 32);
+#pragma unroll
+          for (int k = 0; k < 32; ++k)
+            if (!(seen >> k & 1)) g[k] = 0.f;
+        }
+        span_pack32<T>(g, ds[c]);
+      }
+      tmem_st_32x32b_x16(s_addr, ds[0]);
+      tmem_st_32x32b_x16(s_addr + 16, ds[1]);
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(smem_u32(&ds_ready[wg]));
+    }
+    if (ok && n > 0) {
+      ok = mbar_wait(smem_u32(dq_done), 0, abort_flag, p.status, RB_ERR_TIMEOUT_TMEM_EMPTY);
+      ok = __all_sync(0xffffffffu, ok);
+      tc_fence_after();
+    }
+    if (ok) {
+      // warpgroup w stores columns [w HD / 2, (w + 1) HD / 2)
+      T* out = reinterpret_cast<T*>(p.dq) + b * p.dq_st[0] + row * p.dq_st[1] + h * p.dq_st[2];
+#pragma unroll 1
+      for (int c = 0; c < HD / 64; ++c) {
+        const int d0 = wg * (HD / 2) + c * 32;
+        if (d0 >= p.D) break;
+        uint32_t r[32];
+        if (n > 0) {
+          tmem_ld_32x32b_x32(lane_addr + C::DQ_COL + d0, r);
+          tmem_ld_wait();
+        } else {
+#pragma unroll
+          for (int k = 0; k < 32; ++k) r[k] = 0;
+        }
+        if (!live) continue;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          if (d0 + g * 8 >= p.D) break;
+          uint32_t w[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) w[k] = pack2<T>(__uint_as_float(r[g * 8 + 2 * k]) * p.scale, __uint_as_float(r[g * 8 + 2 * k + 1]) * p.scale);
+          *reinterpret_cast<uint4*>(out + d0 + g * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, 512);
+  }
+}
+
+// ---------------------------------------------------------------- dK, dV
+// A CTA owns 128 keys of one key head and goes over the tiles of 64 query rows, of all query heads that share it, that reach them.  Products run on
+// transposed tiles, S^T [key x row] = K Q^T and dP^T = V dO^T, so that a thread owns a key; P^T (its first 16 columns of 32) and dS^T (the other 16) lie
+// over S^T and are the left operands of dV += P^T dO and dK += dS^T Q.
+template <int HD>
+struct SpanDkvCfg {
+  static constexpr int SUB = HD / 64;
+  static constexpr int KV_SUB = 128 * 128, KV_TILE = SUB * KV_SUB;      // [128 x 64] 16-bit sub-tiles
+  static constexpr int Q_SUB = 64 * 128, Q_TILE = SUB * Q_SUB;
+  static constexpr int STAGES = 4;                                       // Q, dO and 64 rows' {lse2, delta, lo, hi}
+  static constexpr int SMEM_BYTES = 2 * KV_TILE + STAGES * (2 * Q_TILE + 1024) + 1024 + 256;
+  static constexpr int ST_COL = 0, DP_COL = 128, DV_COL = 256, DK_COL = 384;     // S^T, dP^T of buffer w: + 64 w
+};
+
+template <typename T, int HD, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(320, 1)
+    span_dkv_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
+                    const __grid_constant__ CUtensorMap tdo, const SpanBwdParams p) {
+  using C = SpanDkvCfg<HD>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* sK = smem;
+  uint8_t* sV = sK + C::KV_TILE;
+  uint8_t* sQ = sV + C::KV_TILE;                    // [STAGES][Q, dO]
+  uint8_t* sRow = sQ + C::STAGES * 2 * C::Q_TILE;   // [STAGES][lse2 64 | delta 64 | lo 64 | hi 64]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sRow + C::STAGES * 1024);
+  uint64_t *kv_full = bars, *full = bars + 1, *empty = full + C::STAGES, *st_full = empty + C::STAGES, *ready = st_full + 2, *all_done = ready + 2;
+  uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(all_done + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_ptr + 1);
+  __shared__ int s_first, s_last;
+
+  const int warp = uniform_warp_idx(), lane = threadIdx.x & 31;
+  int idx = blockIdx.x;
+  const int kv0 = idx % p.tiles * 128;              // causal: the keys that most rows see first
+  idx /= p.tiles;
+  const int hkv = idx % p.Hkv, b = idx / p.Hkv, group = p.H / p.Hkv;
+  const int off = p.Sk - p.Sq, q_tiles = p.sq_pad / 64;
+  const int4* range = p.range + static_cast<long long>(b) * q_tiles;
+
+  if (threadIdx.x == 0) {
+    prefetch_tensormap(&tq);
+    prefetch_tensormap(&tk);
+    prefetch_tensormap(&tv);
+    prefetch_tensormap(&tdo);
+    mbar_init(smem_u32(kv_full), 1);
+    for (int s = 0; s < C::STAGES; ++s) {
+      mbar_init(smem_u32(&full[s]), 1);
+      mbar_init(smem_u32(&empty[s]), 1);
+    }
+    for (int w = 0; w < 2; ++w) {
+      mbar_init(smem_u32(&st_full[w]), 1);
+      mbar_init(smem_u32(&ready[w]), 256);
+    }
+    mbar_init(smem_u32(all_done), 1);
+    *abort_flag = 0;
+    s_first = 0x7fffffff;
+    s_last = -1;
+    fence_barrier_init();
+  }
+  if (warp == 9) {
+    tmem_alloc(smem_u32(tmem_ptr), 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_ptr;
+  // query tiles from the first to the last that reaches these keys (what lies between and does not is masked)
+  for (int i = threadIdx.x; i < q_tiles; i += 320) {
+    const int4 r = range[i];
+    if (r.x < kv0 + 128 && r.y > kv0) {
+      atomicMin(&s_first, i);
+      atomicMax(&s_last, i);
+    }
+  }
+  __syncthreads();
+  const int tile0 = s_first, per_head = s_last < 0 ? 0 : s_last + 1 - tile0;
+  const int n = per_head * group;
+  auto coords = [&](int it, int& h, int& tile) {
+    const int g = it / per_head;
+    h = hkv * group + g;
+    tile = tile0 + it - g * per_head;
+  };
+
+  if (warp == 8) {
+    // ------------------------------ TMA producer ------------------------------
+    if (lane == 0 && n > 0) {
+      mbar_arrive_expect_tx(smem_u32(kv_full), 2 * C::KV_TILE);
+#pragma unroll
+      for (int s = 0; s < C::SUB; ++s) {
+        tma_load_4d(smem_u32(sK + s * C::KV_SUB), &tk, smem_u32(kv_full), s * 64, kv0, hkv, b);
+        tma_load_4d(smem_u32(sV + s * C::KV_SUB), &tv, smem_u32(kv_full), s * 64, kv0, hkv, b);
+      }
+      bool ok = true;
+      int st = 0;
+      uint32_t ph = 0;
+      for (int it = 0; it < n; ++it) {
+        ok = mbar_wait(smem_u32(&empty[st]), ph ^ 1, abort_flag, p.status, RB_ERR_TIMEOUT_EMPTY);
+        if (!ok) break;
+        int h, tile;
+        coords(it, h, tile);
+        const uint32_t bar = smem_u32(&full[st]), dst = smem_u32(sQ + st * 2 * C::Q_TILE), rows = smem_u32(sRow + st * 1024);
+        mbar_arrive_expect_tx(bar, 2 * C::Q_TILE + 1024);
+        const long long bh = (static_cast<long long>(b) * p.H + h) * p.sq_pad + tile * 64, bb = static_cast<long long>(b) * p.sq_pad + tile * 64;
+        bulk_load_1d(rows, p.row_lse2 + bh, 256, bar);
+        bulk_load_1d(rows + 256, p.row_delta + bh, 256, bar);
+        bulk_load_1d(rows + 512, p.row_lo + bb, 256, bar);
+        bulk_load_1d(rows + 768, p.row_hi + bb, 256, bar);
+#pragma unroll
+        for (int s = 0; s < C::SUB; ++s) {
+          tma_load_4d(dst + s * C::Q_SUB, &tq, bar, s * 64, tile * 64, h, b);
+          tma_load_4d(dst + C::Q_TILE + s * C::Q_SUB, &tdo, bar, s * 64, tile * 64, h, b);
+        }
+        if (++st == C::STAGES) { st = 0; ph ^= 1; }
+      }
+      if (!ok)
+        for (int i = 0; i < 64; ++i) __nanosleep(10000);
+    }
+  } else if (warp == 9) {
+    // ------------------------------ MMA issuer --------------------------------
+    if (n > 0) {
+      constexpr int F = UmmaFormat<T>::value;
+      constexpr uint32_t idesc_st = make_idesc(F, 0, 0, 128, 64), idesc_acc = make_idesc(F, 0, 1, 128, HD);
+      bool ok = mbar_wait(smem_u32(kv_full), 0, abort_flag, p.status, RB_ERR_TIMEOUT_FULL);
+      int st_in = 0, st_out = 0;
+      uint32_t ph_in = 0;
+      auto issue = [&](int it) {        // S^T and dP^T of tile `it`, the next stage
+        ok = mbar_wait(smem_u32(&full[st_in]), ph_in, abort_flag, p.status, RB_ERR_TIMEOUT_FULL);
+        if (!ok) return;
+        tc_fence_after();
+        const uint32_t q = smem_u32(sQ + st_in * 2 * C::Q_TILE);
+        const uint64_t kd = make_smem_desc_sw128(smem_u32(sK), 16, 1024), vd = make_smem_desc_sw128(smem_u32(sV), 16, 1024);
+        const uint64_t qd = make_smem_desc_sw128(q, 16, 1024), dod = make_smem_desc_sw128(q + C::Q_TILE, 16, 1024);
+#pragma unroll
+        for (int s = 0; s < C::SUB; ++s) {
+          umma_f16_w4<2, 2>(tmem_base + C::ST_COL + (it & 1) * 64, kd + s * (C::KV_SUB >> 4), qd + s * (C::Q_SUB >> 4), idesc_st, s != 0);
+          umma_f16_w4<2, 2>(tmem_base + C::DP_COL + (it & 1) * 64, vd + s * (C::KV_SUB >> 4), dod + s * (C::Q_SUB >> 4), idesc_st, s != 0);
+        }
+        umma_commit_w(smem_u32(&st_full[it & 1]));
+        if (++st_in == C::STAGES) { st_in = 0; ph_in ^= 1; }
+      };
+      if (ok) issue(0);
+      for (int it = 0; it < n && ok; ++it) {
+        if (it + 1 < n) issue(it + 1);
+        if (ok) ok = mbar_wait(smem_u32(&ready[it & 1]), (it >> 1) & 1, abort_flag, p.status, RB_ERR_TIMEOUT_FLAG);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t q = smem_u32(sQ + st_out * 2 * C::Q_TILE), pt = tmem_base + C::ST_COL + (it & 1) * 64;
+        // 64 rows are four steps of 16: rows [32 h, 32 h + 32) lie in columns 32 h + {0 .. 15} (P^T) and 32 h + {16 .. 31} (dS^T)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          umma_f16_ts_w(tmem_base + C::DV_COL, pt + (k >> 1) * 32 + (k & 1) * 8, make_smem_desc_sw128(q + C::Q_TILE + k * 2048, C::Q_SUB, 1024), idesc_acc,
+                        (it | k) != 0);
+          umma_f16_ts_w(tmem_base + C::DK_COL, pt + 16 + (k >> 1) * 32 + (k & 1) * 8, make_smem_desc_sw128(q + k * 2048, C::Q_SUB, 1024), idesc_acc,
+                        (it | k) != 0);
+        }
+        umma_commit_w(smem_u32(&empty[st_out]));
+        if (++st_out == C::STAGES) st_out = 0;
+      }
+      if (ok) umma_commit_w(smem_u32(all_done));
+    }
+  } else {
+    // ------------------------------ softmax warps ------------------------------
+    const int t = threadIdx.x & 127, half = warp >> 2;          // key within the tile == TMEM lane; which 32 rows
+    const int kv = kv0 + t;
+    const uint32_t lane_addr = tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    bool ok = true;
+    int st = 0;
+    int4 here = n > 0 ? range[tile0] : make_int4(0, 0, 0, 0);
+    for (int it = 0; it < n; ++it) {
+      int h, tile, h2, tile2 = 0;
+      coords(it, h, tile);
+      const int4 r = here;
+      if (it + 1 < n) {
+        coords(it + 1, h2, tile2);
+        here = range[tile2];
+      }
+      const float slope2 = BIAS ? __ldg(p.c.slopes + h) * kLog2e : 0.f;
+      ok = mbar_wait(smem_u32(&st_full[it & 1]), (it >> 1) & 1, abort_flag, p.status, RB_ERR_TIMEOUT_TMEM_FULL);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tc_fence_after();
+      // the products have read this stage, so its rows' numbers are there; the stage is free only after this tile's last products
+      const uint8_t* rows = sRow + st * 1024 + half * 128;
+      if (++st == C::STAGES) st = 0;
+      const float4 *lse4 = reinterpret_cast<const float4*>(rows), *delta4 = reinterpret_cast<const float4*>(rows + 256);
+      const int4 *lo4 = reinterpret_cast<const int4*>(rows + 512), *hi4 = reinterpret_cast<const int4*>(rows + 768);
+      const bool masked = kv0 < r.z || kv0 + 128 > r.w;
+      const int first = tile * 64 + off;                        // place of the tile's first row among the keys
+      const int side = first >= kv0 + 127 ? 1 : first + 63 <= kv0 ? -1 : 0;
+      const uint32_t st_addr = lane_addr + C::ST_COL + (it & 1) * 64 + half * 32;
+      uint32_t s[32], dp[32], packed[16];
+      float g[32];
+      tmem_ld_32x32b_x32(st_addr, s);
+      tmem_ld_32x32b_x32(lane_addr + C::DP_COL + (it & 1) * 64 + half * 32, dp);
+      tmem_ld_wait();
+      span_scale<CAP, 32>(s, p.c);
+      if constexpr (CAP) span_slip<32>(s, p.inv_out2, g);
+      if constexpr (BIAS) span_bias<1, 32>(s, slope2, (float)(first + half * 32 - kv), side);
+#pragma unroll
+      for (int i4 = 0; i4 < 8; ++i4) {
+        const float4 l = lse4[i4];
+        const float ls[4] = {l.x, l.y, l.z, l.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) s[i4 * 4 + k] = __float_as_uint(fast_exp2(__uint_as_float(s[i4 * 4 + k]) - ls[k]));
+      }
+      uint32_t seen = 0xffffffffu;
+      if (masked) {
+        seen = 0;
+#pragma unroll
+        for (int i4 = 0; i4 < 8; ++i4) {
+          const int4 lo = lo4[i4], hi = hi4[i4];
+          seen |= (kv >= lo.x && kv < hi.x ? 1u : 0u) << (i4 * 4) | (kv >= lo.y && kv < hi.y ? 2u : 0u) << (i4 * 4) |
+                  (kv >= lo.z && kv < hi.z ? 4u : 0u) << (i4 * 4) | (kv >= lo.w && kv < hi.w ? 8u : 0u) << (i4 * 4);
+        }
+#pragma unroll
+        for (int k = 0; k < 32; ++k)
+          if (!(seen >> k & 1)) s[k] = 0;
+      }
+#pragma unroll
+      for (int k = 0; k < 16; ++k) packed[k] = pack2<T>(__uint_as_float(s[2 * k]), __uint_as_float(s[2 * k + 1]));
+      tmem_st_32x32b_x16(st_addr, packed);
+#pragma unroll
+      for (int i4 = 0; i4 < 8; ++i4) {
+        const float4 d = delta4[i4];
+        const float de[4] = {d.x, d.y, d.z, d.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int i = i4 * 4 + k;
+          const float w = CAP ? __uint_as_float(s[i]) * g[i] : __uint_as_float(s[i]);
+          g[i] = w * (__uint_as_float(dp[i]) - de[k]);
+        }
+      }
+      if (masked) {
+#pragma unroll
+        for (int k = 0; k < 32; ++k)
+          if (!(seen >> k & 1)) g[k] = 0.f;
+      }
+      span_pack32<T>(g, packed);
+      tmem_st_32x32b_x16(st_addr + 16, packed);
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(smem_u32(&ready[it & 1]));
+    }
+    if (ok && n > 0) {
+      ok = mbar_wait(smem_u32(all_done), 0, abort_flag, p.status, RB_ERR_TIMEOUT_TMEM_FULL);
+      ok = __all_sync(0xffffffffu, ok);
+      tc_fence_after();
+    }
+    if (ok) {
+      // warps 0-3 store dV, warps 4-7 dK
+      T* out = reinterpret_cast<T*>(half == 0 ? p.dv : p.dk) + b * p.dkv_st[0] + kv * p.dkv_st[1] + hkv * p.dkv_st[2];
+      const float f = half == 0 ? 1.f : p.scale;
+#pragma unroll 1
+      for (int c = 0; c < HD / 32; ++c) {
+        if (c * 32 >= p.D) break;
+        uint32_t r[32];
+        if (n > 0) {
+          tmem_ld_32x32b_x32(lane_addr + (half == 0 ? C::DV_COL : C::DK_COL) + c * 32, r);
+          tmem_ld_wait();
+        } else {                                     // no row sees these keys
+#pragma unroll
+          for (int k = 0; k < 32; ++k) r[k] = 0;
+        }
+        if (kv >= p.Sk) continue;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          if (c * 32 + g * 8 >= p.D) break;
+          uint32_t w[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) w[k] = pack2<T>(__uint_as_float(r[g * 8 + 2 * k]) * f, __uint_as_float(r[g * 8 + 2 * k + 1]) * f);
+          *reinterpret_cast<uint4*>(out + c * 32 + g * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, 512);
+  }
+}
+
+struct SpanBwdMaps {
+  CUtensorMap q, k, v, dout, k64, v64;
+};
+
+template <typename T, int HD, bool CAP, bool BIAS>
+int launch_span_bwd(const SpanBwdMaps& m, SpanBwdParams p, cudaStream_t st) {
+  auto dq = span_dq_kernel<T, HD, CAP, BIAS>;
+  auto dkv = span_dkv_kernel<T, HD, CAP, BIAS>;
+  cudaError_t e = cudaFuncSetAttribute(dq, cudaFuncAttributeMaxDynamicSharedMemorySize, SpanDqCfg<HD>::SMEM_BYTES);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(dkv, cudaFuncAttributeMaxDynamicSharedMemorySize, SpanDkvCfg<HD>::SMEM_BYTES);
+  if (e != cudaSuccess) return 2000 + (int)e;
+  const long long q_tiles = (p.Sq + 127) / 128, kv_tiles = (p.Sk + 127) / 128;
+  if (q_tiles * p.H * p.B > 0x7fffffffll || kv_tiles * p.Hkv * p.B > 0x7fffffffll) return 20;
+  p.tiles = (int)q_tiles;
+  dq<<<(unsigned)(q_tiles * p.H * p.B), 320, SpanDqCfg<HD>::SMEM_BYTES, st>>>(m.k64, m.v64, p);
+  p.tiles = (int)kv_tiles;
+  dkv<<<(unsigned)(kv_tiles * p.Hkv * p.B), 320, SpanDkvCfg<HD>::SMEM_BYTES, st>>>(m.q, m.k, m.v, m.dout, p);
+  e = cudaGetLastError();
+  return e == cudaSuccess ? 0 : 3000 + (int)e;
+}
+
+template <typename T>
+int span_bwd(int dtype, const void* k, const void* v, const long long* ks, const long long* vs, const SpanBwdParams& p, bool cap, cudaStream_t st) {
+  SpanBwdMaps m;
+  int rc = rbh::span_map(&m.q, dtype, p.q, p.q_st, p.B, p.Sq, p.H, p.D, 64);
+  if (!rc) rc = rbh::span_map(&m.dout, dtype, p.dout, p.do_st, p.B, p.Sq, p.H, p.D, 64);
+  if (!rc) rc = rbh::span_map(&m.k, dtype, k, ks, p.B, p.Sk, p.Hkv, p.D, 128);
+  if (!rc) rc = rbh::span_map(&m.v, dtype, v, vs, p.B, p.Sk, p.Hkv, p.D, 128);
+  if (!rc) rc = rbh::span_map(&m.k64, dtype, k, ks, p.B, p.Sk, p.Hkv, p.D, 64);
+  if (!rc) rc = rbh::span_map(&m.v64, dtype, v, vs, p.B, p.Sk, p.Hkv, p.D, 64);
+  if (rc) return 1000 + rc;
+  const bool bias = p.c.slopes != nullptr;
+#define RB_SPAN(HD_)                                                                                               \
+  (cap ? bias ? launch_span_bwd<T, HD_, true, true>(m, p, st) : launch_span_bwd<T, HD_, true, false>(m, p, st)     \
+       : bias ? launch_span_bwd<T, HD_, false, true>(m, p, st) : launch_span_bwd<T, HD_, false, false>(m, p, st))
+  return p.D <= 64 ? RB_SPAN(64) : RB_SPAN(128);
+#undef RB_SPAN
+}
+
+}  // namespace rb
+
+extern "C" {
+
+// Gradients of rb_span_fwd.  q, k, v, dout: 16-bit views as there; o contiguous and lse2 from the forward call with the same arguments.  dq [B, Sq, H, D]; dk and
+// dv [B, Sk, Hkv, D] of the same strides: views of 16-byte aligned rows.  scratch: 16-byte aligned, B pad (8 H + 8) + B pad / 4 bytes with pad = Sq rounded up to
+// a multiple of 64; nothing in it has to be set.
+int rb_span_bwd(int dtype, const void* q, const void* k, const void* v, const long long* qs, const long long* ks, const long long* vs, const int* spans,
+                long long span_batch, const float* slopes, const void* o, const float* lse2, const void* dout, const long long* dos, void* scratch, void* dq,
+                void* dk, void* dv, const long long* dqs, const long long* dkvs, int B, int H, int Hkv, int Sq, int Sk, int D, int causal, float scale,
+                float cap, void* stream) {
+  using namespace rb;
+  if (B <= 0 || H <= 0 || Sq <= 0) return 0;
+  if (Sk <= 0 || Hkv <= 0 || H % Hkv || D <= 0 || D > 128 || D % 8 || Sq > 0x7fffffff - 128) return 20;
+  SpanBwdParams p{};
+  p.B = B; p.H = H; p.Hkv = Hkv; p.Sq = Sq; p.Sk = Sk; p.D = D;
+  p.c.scale2 = scale * kLog2e;
+  p.c.in = cap > 0.f ? scale / cap : 0.f;
+  p.c.out2 = cap * kLog2e;
+  p.c.slopes = slopes;
+  p.c.spans = reinterpret_cast<const int2*>(spans);
+  p.c.span_batch = span_batch;
+  p.c.causal = causal;
+  p.scale = scale;
+  p.inv_out2 = cap > 0.f ? 1.f / p.c.out2 : 0.f;
+  p.q = q; p.o = o; p.dout = dout; p.lse2 = lse2;
+  for (int i = 0; i < 3; ++i) { p.q_st[i] = qs[i]; p.do_st[i] = dos[i]; p.dq_st[i] = dqs[i]; p.dkv_st[i] = dkvs[i]; }
+  p.sq_pad = (Sq + 63) / 64 * 64;
+  const long long rows = static_cast<long long>(B) * p.sq_pad;
+  p.row_lse2 = reinterpret_cast<float*>(scratch);
+  p.row_delta = p.row_lse2 + rows * H;
+  p.row_lo = reinterpret_cast<int*>(p.row_delta + rows * H);
+  p.row_hi = p.row_lo + rows;
+  p.range = reinterpret_cast<int4*>(p.row_hi + rows);
+  p.dq = dq; p.dk = dk; p.dv = dv;
+  p.status = rbh::device_status_word();
+  cudaStream_t st = (cudaStream_t)stream;
+  if (dtype == rbh::DT_BF16) return span_bwd<__nv_bfloat16>(dtype, k, v, ks, vs, p, cap > 0.f, st);
+  if (dtype == rbh::DT_F16) return span_bwd<__half>(dtype, k, v, ks, vs, p, cap > 0.f, st);
+  return 20;
+}
+}

@@ -678,6 +678,19 @@ def flash_attention(q, k, v, causal: bool = True, scale: Optional[float] = None)
     return sdpa_reference(q, k, v, causal, scale)
 
 
+def span_attention(q, k, v, spans=None, causal: bool = True, scale: Optional[float] = None, cap: float = 0.0, slopes=None):
+    """Attention on ``[B, S, H, d]`` tensors whose scores are capped (``cap tanh(s / cap)``) and fall with the distance (``slopes`` per head), and whose
+    rows see a span of keys each (``spans [B, S, 2]``: packed documents, prefixes, windows, padding).  See ``ops/span.py``."""
+    from .span import span_attention as _span
+    return _span(q, k, v, spans, causal, scale, cap, slopes)
+
+
+def document_spans(documents, prefix=None, causal: bool = True):
+    """Spans of packed documents for ``span_attention``; see ``ops/span.py``."""
+    from .span import document_spans as _spans
+    return _spans(documents, prefix, causal)
+
+
 def _sdpa_composed(q, k, v, causal, scale):
     """fp32 CUDA tensors: batched matmul + softmax kernels (the reference's composition,
     rumus/src/nn/attention.rs:17-58)."""

@@ -1,0 +1,335 @@
+"""Span attention: scores that are capped by a tanh and fall with the distance, rows that see a span of keys each.
+
+    x_ij = cap tanh(scale q_i.k_j / cap) - slope_h |i + Sk - Sq - j|      (either part may be missing)
+    row i sees the keys lo_i <= j < hi_i, with ``causal`` none behind its own place i + Sk - Sq
+    o_i = sum_j softmax(x_i)_j v_j                                         (zeros for a row that sees no key)
+
+Spans cover packed documents, prompts whose beginning is seen by all of it, windows and padding (``document_spans``).  On a GPU one kernel forward and
+two backward (``csrc/kernels/span_attention_{fwd,bwd}.cu``) and one for a new token over pages (``span_decode.cu``); on a CPU plain math.  Gradients are
+summed in a fixed order: the same inputs give the same gradients.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from contextlib import nullcontext
+from ctypes import c_float, c_int, c_longlong, c_void_p
+from typing import Optional
+
+import torch
+
+from . import native
+from ._lib import check, count_launch, ptr, stream_ptr
+
+P, LL, I, Fl = c_void_p, c_longlong, c_int, c_float
+native.register_signature("rb_span_fwd_splits", [I, I, I, I])
+native.register_signature("rb_span_fwd", [I] + [P] * 7 + [LL] + [P] * 5 + [I] * 8 + [Fl, Fl, P])
+native.register_signature("rb_span_bwd", [I] + [P] * 7 + [LL] + [P] * 11 + [I] * 7 + [Fl, Fl, P])
+native.register_signature("rb_span_decode_splits", [I, I, I, I])
+native.register_signature("rb_span_decode", [I, I, P, LL, LL] + [P] * 9 + [I] * 8 + [Fl, Fl, P])
+
+CLUSTER = 8             # parts of a context that one launch joins (kSdCluster)
+HALVES = (torch.bfloat16, torch.float16)
+
+
+# ---------------------------------------------------------------- spans and slopes
+def document_spans(documents: torch.Tensor, prefix: Optional[torch.Tensor] = None, causal: bool = True) -> torch.Tensor:
+    """Spans ``int32 [B, S, 2]`` of packed documents.  ``documents``: ``[B, S]`` whole numbers, equal for neighbouring tokens of one document, negative
+    for padding (sees nothing, is seen by none).  A token sees its own document: all of it, with ``causal`` up to itself.  ``prefix``: ``[B, S]``
+    truth values; with ``causal`` a document's tokens up to the last of its leading run of them see one another (and all later ones of the document
+    see them)."""
+    if documents.dim() != 2 or documents.dtype.is_floating_point or documents.dtype == torch.bool:
+        raise ValueError(f"documents are whole numbers [B, S], not {documents.dtype} {tuple(documents.shape)}")
+    B, S = documents.shape
+    place = torch.arange(S, device=documents.device).expand(B, S)
+    if S == 0:
+        return torch.zeros((B, 0, 2), dtype=torch.int32, device=documents.device)
+    new = torch.ones((B, S), dtype=torch.bool, device=documents.device)
+    new[:, 1:] = documents[:, 1:] != documents[:, :-1]
+    lo = torch.where(new, place, 0).cummax(1).values
+    last = torch.ones_like(new)
+    last[:, :-1] = new[:, 1:]
+    end = torch.where(last, place + 1, S).flip(1).cummin(1).values.flip(1)
+    hi = torch.minimum(end, place + 1) if causal else end
+    if prefix is not None:
+        if prefix.shape != documents.shape or prefix.dtype != torch.bool or prefix.device != documents.device:
+            raise ValueError(f"a prefix is truth values of the documents' shape {tuple(documents.shape)}, not {prefix.dtype} {tuple(prefix.shape)}")
+        # the first token of each document that is no prefix: the least such place at or behind the document's beginning
+        stop = torch.where(prefix, S, place).flip(1).cummin(1).values.flip(1)
+        hi = torch.maximum(hi, torch.minimum(stop.gather(1, lo), end))
+    there = documents >= 0
+    return torch.stack([torch.where(there, lo, 0), torch.where(there, hi, 0)], -1).to(torch.int32)
+
+
+def distance_slopes(heads: int, device=None) -> torch.Tensor:
+    """``fp32 [heads]``: 2^(-8 (h + 1) / heads), the geometric slopes of linear distance biases."""
+    if heads <= 0:
+        raise ValueError(f"{heads} heads")
+    return torch.tensor([2.0 ** (-8.0 * (h + 1) / heads) for h in range(heads)], dtype=torch.float32, device=device)
+
+
+# ---------------------------------------------------------------- arguments
+def _scores_ok(heads: int, device, scale: float, cap: float, slopes) -> None:
+    if not math.isfinite(scale):
+        raise ValueError(f"scale {scale}")
+    if not (math.isfinite(cap) and cap >= 0.0):
+        raise ValueError(f"a cap is a number above zero, or zero for none, not {cap}")
+    if slopes is not None:
+        if slopes.dtype != torch.float32 or tuple(slopes.shape) != (heads,) or slopes.device != device:
+            raise ValueError(f"slopes are float32 [{heads}] on {device}, not {slopes.dtype} {tuple(slopes.shape)} on {slopes.device}")
+        if slopes.requires_grad:
+            raise ValueError("slopes are constants: span attention has no gradient for them")
+
+
+def _rows_ok(q, k, v, spans, scale, cap, slopes) -> None:
+    if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape:
+        raise ValueError(f"span attention of {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    B, Sq, H, D = q.shape
+    Bk, Sk, Hkv, Dk = k.shape
+    if Bk != B or Dk != D or D == 0 or H == 0 or Hkv == 0 or H % Hkv:
+        raise ValueError(f"span attention of heads {tuple(q.shape)} over {tuple(k.shape)}")
+    if not (q.dtype == k.dtype == v.dtype and q.device == k.device == v.device):
+        raise ValueError(f"span attention of {q.dtype}, {k.dtype}, {v.dtype} on {q.device}, {k.device}, {v.device}")
+    if not q.dtype.is_floating_point:
+        raise TypeError(f"span attention of {q.dtype}")
+    if spans is not None:
+        if spans.dtype != torch.int32 or tuple(spans.shape) not in ((B, Sq, 2), (Sq, 2)) or spans.device != q.device:
+            raise ValueError(f"spans are int32 [{B}, {Sq}, 2] or [{Sq}, 2] on {q.device}, not {spans.dtype} {tuple(spans.shape)} on {spans.device}")
+    _scores_ok(H, q.device, scale, cap, slopes)
+
+
+def kernels_take(q: torch.Tensor) -> bool:
+    """Whether the GPU kernels cover heads of this type and size."""
+    return q.dtype in HALVES and q.shape[-1] % 8 == 0 and 0 < q.shape[-1] <= 128
+
+
+def _on(device):
+    """Makes ``device`` the current one: launches go to its current stream."""
+    return nullcontext() if device.index in (None, torch.cuda.current_device()) else torch.cuda.device(device)
+
+
+def _strides(t: torch.Tensor):
+    """{batch, row, head} strides of a view as the launchers take them.  A dimension of one element has any stride; the tensor maps want a multiple
+    of 16 bytes."""
+    return (LL * 3)(*(t.stride(i) if t.shape[i] > 1 else t.shape[3] for i in range(3)))
+
+
+def _view_ok(t: torch.Tensor) -> bool:
+    """Whether the kernels read this view in place: rows of neighbouring numbers, 16-byte aligned, no dimension that repeats."""
+    return (t.stride(3) == 1 or t.shape[3] == 1) and t.data_ptr() % 16 == 0 and all(
+        t.shape[i] == 1 or (t.stride(i) > 0 and t.stride(i) % 8 == 0 and t.stride(i) < 2 ** 39) for i in range(3))
+
+
+def _view(t: torch.Tensor) -> torch.Tensor:
+    return t if _view_ok(t) else t.clone(memory_format=torch.contiguous_format)
+
+
+def _spans_arg(spans, rows: int):
+    """(contiguous spans, rows from one batch's to the next's)."""
+    if spans is None:
+        return None, 0
+    return spans.contiguous(), rows if spans.dim() == 3 else 0
+
+
+# ---------------------------------------------------------------- kernels
+def span_forward(q, k, v, spans, causal: bool, scale: float, cap: float, slopes, out=None):
+    """Heads ``[B, Sq, H, D]`` and the rows' log-sum-exp in units of log 2 ``[B, H, Sq]``.  ``out``: contiguous tensor to write into."""
+    B, Sq, H, D = q.shape
+    Sk, Hkv = k.shape[1], k.shape[2]
+    o = out if out is not None else torch.empty((B, Sq, H, D), dtype=q.dtype, device=q.device)
+    if not o.is_contiguous() or o.shape != q.shape or o.dtype != q.dtype or o.device != q.device or o.data_ptr() % 16:
+        raise ValueError(f"span attention writes contiguous heads {tuple(q.shape)} of {q.dtype}, not {o.dtype} {tuple(o.shape)}")
+    lse2 = torch.empty((B, H, Sq), dtype=torch.float32, device=q.device)
+    if o.numel() == 0:
+        return o, lse2
+    if Sk == 0:
+        return o.zero_(), lse2.fill_(float("-inf"))
+    spans, batch = _spans_arg(spans, Sq)
+    slopes = None if slopes is None else slopes.contiguous()
+    with _on(q.device):
+        L = native.lib()
+        splits = L.rb_span_fwd_splits(B, H, Sq, Sk)
+        part_o = part_lse2 = None
+        if splits > 1:
+            part_o = torch.empty((splits, B, Sq, H, D), dtype=torch.float32, device=q.device)
+            part_lse2 = torch.empty((splits, B, H, Sq), dtype=torch.float32, device=q.device)
+        st = [_strides(t) for t in (q, k, v)]
+        check(L.rb_span_fwd(native.dtype_code(q.dtype), ptr(q), ptr(k), ptr(v), *map(ctypes.addressof, st), ptr(spans), batch, ptr(slopes), ptr(o),
+                            ptr(lse2), ptr(part_o), ptr(part_lse2), B, H, Hkv, Sq, Sk, D, splits, int(causal), float(scale), float(cap),
+                            stream_ptr()), "rb_span_fwd")
+        count_launch(2 if splits > 1 else 1)
+    return o, lse2
+
+
+def span_backward(q, k, v, spans, causal: bool, scale: float, cap: float, slopes, o, lse2, dout, out=None):
+    """dq, dk, dv.  ``out``: views of 16-byte aligned rows to write them into (dk and dv of the same strides)."""
+    B, Sq, H, D = q.shape
+    Sk, Hkv = k.shape[1], k.shape[2]
+    dq, dk, dv = out if out is not None else (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+    if q.numel() == 0 or k.numel() == 0:
+        return dq.zero_(), dk.zero_(), dv.zero_()
+    dout = _view(dout)
+    spans, batch = _spans_arg(spans, Sq)
+    slopes = None if slopes is None else slopes.contiguous()
+    with _on(q.device):
+        L = native.lib()
+        rows = B * ((Sq + 63) // 64) * 64
+        scratch = torch.empty(rows * (8 * H + 8) + rows // 64 * 16, dtype=torch.uint8, device=q.device)
+        st = [_strides(t) for t in (q, k, v)]
+        rest = [_strides(t) for t in (dout, dq, dk)]
+        at = [ctypes.addressof(s) for s in rest]
+        check(L.rb_span_bwd(native.dtype_code(q.dtype), ptr(q), ptr(k), ptr(v), *map(ctypes.addressof, st), ptr(spans), batch, ptr(slopes), ptr(o),
+                            ptr(lse2), ptr(dout), at[0], ptr(scratch), ptr(dq), ptr(dk), ptr(dv), at[1], at[2], B, H, Hkv, Sq, Sk, D, int(causal),
+                            float(scale), float(cap), stream_ptr()), "rb_span_bwd")
+        count_launch(2)
+    return dq, dk, dv
+
+
+class _SpanAttnFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, spans, causal, scale, cap, slopes):
+        q, k, v = _view(q), _view(k), _view(v)
+        o, lse2 = span_forward(q, k, v, spans, causal, scale, cap, slopes)
+        ctx.args = causal, scale, cap
+        ctx.save_for_backward(q, k, v, spans, slopes, o, lse2)
+        return o
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        q, k, v, spans, slopes, o, lse2 = ctx.saved_tensors
+        causal, scale, cap = ctx.args
+        return (*span_backward(q, k, v, spans, causal, scale, cap, slopes, o, lse2, dout), None, None, None, None, None)
+
+
+# ---------------------------------------------------------------- plain math
+def _weights(raw, distance, seen, slopes, cap: float):
+    """Softmax weights of scaled products ``[..., heads, rows, keys]``; rows that see nothing get zeros."""
+    if cap > 0:
+        raw = torch.tanh(raw / cap) * cap
+    if slopes is not None:
+        raw = raw - slopes.to(raw.dtype).view(-1, 1, 1) * distance
+    top = raw.masked_fill(~seen, -math.inf).amax(-1, keepdim=True) if raw.shape[-1] else raw.new_zeros(raw.shape[:-1] + (1,))
+    # masked places take part as zeros, not as exp(-inf - ...): their gradient is zero too, and rows without keys stay finite
+    w = torch.exp(torch.where(seen, raw - torch.where(top.isinf(), 0.0, top).detach(), -math.inf))
+    total = w.sum(-1, keepdim=True)
+    return w / torch.where(total > 0, total, 1.0)
+
+
+def span_reference(q, k, v, spans=None, causal: bool = True, scale: Optional[float] = None, cap: float = 0.0, slopes=None):
+    """The same in plain math (32 bits inside; 64-bit tensors stay so)."""
+    B, Sq, H, D = q.shape
+    Sk, Hkv = k.shape[1], k.shape[2]
+    scale = scale if scale is not None else 1.0 / math.sqrt(D)
+    acc = torch.float64 if q.dtype == torch.float64 else torch.float32
+    qf, kf, vf = (t.to(acc).transpose(1, 2) for t in (q, k, v))
+    if Hkv != H:
+        kf, vf = (t.repeat_interleave(H // Hkv, dim=1) for t in (kf, vf))
+    place, key = torch.arange(Sq, device=q.device)[:, None] + (Sk - Sq), torch.arange(Sk, device=q.device)
+    seen = torch.ones((1, 1, Sq, Sk), dtype=torch.bool, device=q.device)
+    if causal:
+        seen = seen & (key <= place)
+    if spans is not None:
+        lo, hi = spans.reshape(-1, 1, Sq, 1, 2).unbind(-1)
+        seen = seen & (key >= lo) & (key < hi)
+    w = _weights((qf @ kf.transpose(-1, -2)) * scale, (place - key).abs().to(acc), seen, slopes, cap)
+    return (w @ vf).transpose(1, 2).to(q.dtype)
+
+
+# ---------------------------------------------------------------- entry points
+def span_attention(q, k, v, spans=None, causal: bool = True, scale: Optional[float] = None, cap: float = 0.0, slopes=None):
+    """Span attention of ``q [B, Sq, H, D]`` over ``k, v [B, Sk, Hkv, D]`` (``Hkv`` divides ``H``; strided views are fine), differentiable in q, k and v.
+
+    ``spans``: int32 ``[B, Sq, 2]`` (or ``[Sq, 2]`` for all batches), row i sees the keys ``lo <= j < hi``; parts outside the keys count as cut off, and
+    a row with ``hi <= lo`` gives zeros.  ``causal``: besides, no key behind place ``i + Sk - Sq``.  ``cap``: scores s become cap tanh(s / cap), 0: they
+    stay.  ``slopes``: float32 ``[H]``, what a score loses per place of distance (constants).  Keys and values have to be finite, unseen ones too: a
+    weight of zero times what is not finite is not a number.  On a GPU: bfloat16 or float16, D a multiple of 8 up to 128."""
+    scale = float(scale) if scale is not None else 1.0 / math.sqrt(q.shape[-1])
+    cap = float(cap)
+    _rows_ok(q, k, v, spans, scale, cap, slopes)
+    if not q.is_cuda:
+        return span_reference(q, k, v, spans, causal, scale, cap, slopes)
+    if not kernels_take(q):
+        raise TypeError(f"span attention on a GPU takes bfloat16 or float16 heads of a multiple of 8 numbers up to 128, not {q.dtype} of {q.shape[-1]}")
+    return _SpanAttnFn.apply(q, k, v, spans, bool(causal), scale, cap, slopes)
+
+
+def span_decode(q, k_cache, v_cache, block_tables, ctx_lens, max_ctx: int, scale: Optional[float] = None, cap: float = 0.0, slopes=None, starts=None,
+                head_major: bool = False, out=None):
+    """Span attention of one token per sequence over pages: ``q [B, H, D]`` sees the tokens ``starts[b] <= t < ctx_lens[b]`` of its sequence, itself the
+    last of them; returns ``[B, H, D]`` (zeros where it sees none).
+
+    Caches ``[pages, page, Hkv, D]``, with ``head_major`` ``[pages, Hkv, page, D]``; ``block_tables`` int32 ``[B, n]``; ``ctx_lens``, ``starts`` (None:
+    0) int32 ``[B]``; ``max_ctx``: no context is longer (decides how contexts are cut; longer ones are still right).  Tokens in pages that the cache
+    does not have, and behind the table's end, count as unseen; what pages hold behind a context is never read.  ``cap``, ``slopes``: as in
+    ``span_attention``.  ``out``: contiguous tensor to write into.  On a GPU: bfloat16 or float16, D a multiple of 8 up to 128."""
+    if q.dim() != 3 or k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
+        raise ValueError(f"decoding of {tuple(q.shape)} over pages {tuple(k_cache.shape)}, {tuple(v_cache.shape)}")
+    B, H, D = q.shape
+    pages, (Hkv, page) = k_cache.shape[0], ((k_cache.shape[1], k_cache.shape[2]) if head_major else (k_cache.shape[2], k_cache.shape[1]))
+    if k_cache.shape[3] != D or D == 0 or H == 0 or Hkv == 0 or page == 0 or H % Hkv:
+        raise ValueError(f"decoding of heads {tuple(q.shape)} over pages {tuple(k_cache.shape)}")
+    if not (q.dtype == k_cache.dtype == v_cache.dtype and q.device == k_cache.device == v_cache.device):
+        raise ValueError(f"decoding of {q.dtype}, {k_cache.dtype}, {v_cache.dtype} on {q.device}, {k_cache.device}, {v_cache.device}")
+    if not q.dtype.is_floating_point:
+        raise TypeError(f"decoding of {q.dtype}")
+    ints = [("block_tables", block_tables, 2), ("ctx_lens", ctx_lens, 1)] + ([] if starts is None else [("starts", starts, 1)])
+    for name, t, dim in ints:
+        if t.dtype != torch.int32 or t.dim() != dim or t.shape[0] != B or t.device != q.device:
+            raise ValueError(f"{name}: int32 of {dim} dimensions for {B} sequences on {q.device}, not {t.dtype} {tuple(t.shape)} on {t.device}")
+    if max_ctx < 0:
+        raise ValueError(f"max_ctx {max_ctx}")
+    scale = float(scale) if scale is not None else 1.0 / math.sqrt(D)
+    cap = float(cap)
+    _scores_ok(H, q.device, scale, cap, slopes)
+    if out is None:
+        out = torch.empty((B, H, D), dtype=q.dtype, device=q.device)
+    elif not out.is_contiguous() or out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or out.data_ptr() % 8:
+        raise ValueError(f"decoding writes contiguous heads {tuple(q.shape)} of {q.dtype}, not {out.dtype} {tuple(out.shape)}")
+    if not q.is_cuda:
+        return out.copy_(_decode_reference(q, k_cache, v_cache, block_tables, ctx_lens, scale, cap, slopes, starts, head_major))
+    if not kernels_take(q):
+        raise TypeError(f"decoding on a GPU takes bfloat16 or float16 heads of a multiple of 8 numbers up to 128, not {q.dtype} of {D}")
+    if not k_cache.is_contiguous() or not v_cache.is_contiguous() or k_cache.data_ptr() % 16 or v_cache.data_ptr() % 16:
+        raise ValueError("the caches' pages are contiguous and 16-byte aligned")
+    if out.numel() == 0:
+        return out
+    if q.stride(2) != 1 or q.stride(1) % 2 or q.stride(0) % 2 or q.data_ptr() % 4:
+        q = q.clone(memory_format=torch.contiguous_format)
+    block_tables, ctx_lens = block_tables.contiguous(), ctx_lens.contiguous()
+    starts = None if starts is None else starts.contiguous()
+    slopes = None if slopes is None else slopes.contiguous()
+    with _on(q.device):
+        L = native.lib()
+        splits = L.rb_span_decode_splits(B, H, Hkv, min(int(max_ctx), block_tables.shape[1] * page, 0x7fffffff))
+        part_o = part_lse2 = None
+        if splits > CLUSTER:
+            part_o = torch.empty((splits, B, H, D), dtype=torch.float32, device=q.device)
+            part_lse2 = torch.empty((splits, B, H), dtype=torch.float32, device=q.device)
+        check(L.rb_span_decode(native.dtype_code(q.dtype), int(head_major), ptr(q), q.stride(0), q.stride(1), ptr(k_cache), ptr(v_cache),
+                               ptr(block_tables), ptr(ctx_lens), ptr(starts), ptr(slopes), ptr(out), ptr(part_o), ptr(part_lse2), B, H, Hkv, D, page,
+                               pages, block_tables.shape[1], splits, scale, cap, stream_ptr()), "rb_span_decode")
+        count_launch(2 if splits > CLUSTER else 1)
+    return out
+
+
+def _decode_reference(q, k_cache, v_cache, block_tables, ctx_lens, scale, cap, slopes, starts, head_major):
+    B, H, D = q.shape
+    pages, page = k_cache.shape[0], k_cache.shape[2 if head_major else 1]
+    acc = torch.float64 if q.dtype == torch.float64 else torch.float32
+    outs = torch.zeros((B, H, D), dtype=acc, device=q.device)
+    for b in range(B):
+        n = min(int(ctx_lens[b]), block_tables.shape[1] * page)
+        t = torch.arange(max(0 if starts is None else int(starts[b]), 0), max(n, 0), device=q.device)
+        if t.numel() == 0:
+            continue
+        blk = block_tables[b, t // page].long()
+        there = (blk >= 0) & (blk < pages)
+        t, blk = t[there], blk[there]
+        kk, vv = ((c[blk, :, t % page] if head_major else c[blk, t % page]).to(acc) for c in (k_cache, v_cache))    # [n, Hkv, D]
+        rep = H // kk.shape[1]
+        kk, vv = kk.repeat_interleave(rep, 1).transpose(0, 1), vv.repeat_interleave(rep, 1).transpose(0, 1)
+        raw = (q[b].to(acc)[:, None] @ kk.transpose(1, 2)) * scale
+        w = _weights(raw, (int(ctx_lens[b]) - 1 - t).to(acc), torch.ones_like(raw, dtype=torch.bool), slopes, cap)
+        outs[b] = (w @ vv)[:, 0]
+    return outs.to(q.dtype)
