@@ -16,14 +16,14 @@ namespace rb {
 
 struct SpanBwdParams {
   int B, H, Hkv, Sq, Sk, D;
-  int tiles;                        // of the launch, along rows or keys
+  SpanOrder order;                  // of the launch: tiles of rows and heads, or tiles of keys and key heads
   SpanScores c;
-  float scale, inv_out2;            // 1 / (cap log2 e)
+  float grad_scale;                 // scale, negated with a cap (span_score32 gives its derivative negated)
   const void *q, *o, *dout;         // o [B, Sq, H, D] contiguous
   long long q_st[3], do_st[3];
   const float* lse2;                // [B, H, Sq]
   // per row, rows padded to a multiple of 64 (zeros there)
-  float *row_lse2, *row_delta;      // [B, H, sq_pad]
+  float *row_lse2, *row_delta;      // [B, H, sq_pad], both negated
   int *row_lo, *row_hi;             // [B, sq_pad]
   int4* range;                      // [B, sq_pad / 64] {least lo, largest hi, largest lo, least hi}
   int sq_pad;
@@ -33,22 +33,9 @@ struct SpanBwdParams {
 };
 
 template <typename T>
-__device__ __forceinline__ void span_pack32(const float* f, uint32_t* w) {
+__device__ __forceinline__ void span_pack32(const uint32_t* f, uint32_t* w) {
 #pragma unroll
-  for (int i = 0; i < 16; ++i) w[i] = pack2<T>(f[2 * i], f[2 * i + 1]);
-}
-
-// 1 - t^2 of capped scores (log2 units), in place of which the caller goes on with the scores
-template <int N>
-__device__ __forceinline__ void span_slip(const uint32_t* s, float inv_out2, float* slip) {
-  const uint64_t k = f32x2(inv_out2, inv_out2), one = f32x2(1.f, 1.f), minus = f32x2(-1.f, -1.f);
-#pragma unroll
-  for (int i = 0; i < N; i += 2) {
-    const uint64_t t = mul_f32x2(f32x2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), k);
-    const float2 v = f32x2_get(fma_f32x2(mul_f32x2(t, minus), t, one));
-    slip[i] = v.x;
-    slip[i + 1] = v.y;
-  }
+  for (int i = 0; i < 16; ++i) w[i] = pack2<T>(__uint_as_float(f[2 * i]), __uint_as_float(f[2 * i + 1]));
 }
 
 // ---------------------------------------------------------------- dQ
@@ -76,10 +63,9 @@ __global__ void __launch_bounds__(320, 1)
   __shared__ float s_delta[128];
 
   const int warp = uniform_warp_idx(), lane = threadIdx.x & 31;
-  int idx = blockIdx.x;
-  const int q0 = (p.tiles - 1 - idx % p.tiles) * 128;                                  // causal: the longest first
-  idx /= p.tiles;
-  const int h = idx % p.H, b = idx / p.H, hkv = h / (p.H / p.Hkv);
+  int tile, unit;
+  span_place<true>(p.order, blockIdx.x, tile, unit);
+  const int q0 = tile * 128, h = unit % p.H, b = unit / p.H, hkv = h / (p.H / p.Hkv);
   const int off = p.Sk - p.Sq;
   const int t = threadIdx.x & 127, wg = warp >> 2, row = q0 + t;
   const bool live = row < p.Sq;
@@ -148,8 +134,8 @@ __global__ void __launch_bounds__(320, 1)
     if (live && span.x < span.y) lse2 = p.lse2[(static_cast<long long>(b) * p.H + h) * p.Sq + row];
     if (row < p.sq_pad) {
       const long long at = (static_cast<long long>(b) * p.H + h) * p.sq_pad + row;
-      if (wg == 0) p.row_lse2[at] = lse2;
-      else p.row_delta[at] = delta;
+      if (wg == 0) p.row_lse2[at] = -lse2;
+      else p.row_delta[at] = -delta;
       if (h == 0 && wg == 0) {
         p.row_lo[static_cast<long long>(b) * p.sq_pad + row] = span.x;
         p.row_hi[static_cast<long long>(b) * p.sq_pad + row] = span.y;
@@ -233,32 +219,33 @@ __global__ void __launch_bounds__(320, 1)
       tc_fence_after();
       const int kv0 = (j0 + i) * 64;
       const bool masked = kv0 < all.z || kv0 + 64 > all.w;
-      const int side = q0 + off >= kv0 + 63 ? 1 : q0 + 127 + off <= kv0 ? -1 : 0;
+      const int side = !BIAS ? 1 : p.c.causal || q0 + off >= kv0 + 63 ? 1 : q0 + 127 + off <= kv0 ? -1 : 0;
+      const float slope = side > 0 ? slope2 : -slope2;
+      const uint64_t minus = both(-delta);
       uint32_t ds[2][16];
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        uint32_t s[32], dp[32];
-        float g[32];
+        uint32_t s[32], dp[32], slip[32];
         tmem_ld_32x32b_x32(s_addr + c * 32, s);
         tmem_ld_32x32b_x32(dp_addr + c * 32, dp);
         tmem_ld_wait();
-        span_scale<CAP, 32>(s, p.c);
-        if constexpr (CAP) span_slip<32>(s, p.inv_out2, g);
-        if constexpr (BIAS) span_bias<-1, 32>(s, slope2, (float)(row + off - kv0 - c * 32), side);
-#pragma unroll
-        for (int k = 0; k < 32; ++k) {
-          const float w = fast_exp2(__uint_as_float(s[k]) - lse2);
-          g[k] = CAP ? w * g[k] : w;
+        const uint32_t seen = masked ? span_bits(span.x - kv0 - c * 32, span.y - kv0 - c * 32) : 0xffffffffu;
+        if (masked) span_mask32(s, seen, 0);         // what unseen keys hold decides nothing
+        const float first = (float)(row + off - kv0 - c * 32), reach = CAP ? span_reach32(s) : 0.f;
+        if (BIAS && side != 0) {
+          span_score32<CAP, true>(s, p.c, SpanAdd<true, false>({fmaf(-slope, first, -lse2), slope}, nullptr), slip, reach);
+        } else {
+          span_score32<CAP, true>(s, p.c, SpanAdd<false, false>({-lse2, 0.f}, nullptr), slip, reach);
+          if constexpr (BIAS) span_both_sides32<-1>(s, slope2, first);
         }
 #pragma unroll
-        for (int k = 0; k < 32; ++k) g[k] *= __uint_as_float(dp[k]) - delta;
-        if (masked) {
-          const uint32_t seen = span_bits(span.x - kv0 - c * 32, span.y - kv0 - c * 32);
-#pragma unroll
-          for (int k = 0; k < 32; ++k)
-            if (!(seen >> k & 1)) g[k] = 0.f;
+        for (int k = 0; k < 32; k += 2) {
+          uint64_t w = f32x2(fast_exp2(__uint_as_float(s[k])), fast_exp2(__uint_as_float(s[k + 1])));
+          if (CAP) w = mul_f32x2(w, pair_at(slip, k));
+          set_pair(s, k, mul_f32x2(w, add_f32x2(pair_at(dp, k), minus)));
         }
-        span_pack32<T>(g, ds[c]);
+        if (masked) span_mask32(s, seen, 0);
+        span_pack32<T>(s, ds[c]);
       }
       tmem_st_32x32b_x16(s_addr, ds[0]);
       tmem_st_32x32b_x16(s_addr + 16, ds[1]);
@@ -292,7 +279,7 @@ __global__ void __launch_bounds__(320, 1)
           if (d0 + g * 8 >= p.D) break;
           uint32_t w[4];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) w[k] = pack2<T>(__uint_as_float(r[g * 8 + 2 * k]) * p.scale, __uint_as_float(r[g * 8 + 2 * k + 1]) * p.scale);
+          for (int k = 0; k < 4; ++k) w[k] = pack2<T>(__uint_as_float(r[g * 8 + 2 * k]) * p.grad_scale, __uint_as_float(r[g * 8 + 2 * k + 1]) * p.grad_scale);
           *reinterpret_cast<uint4*>(out + d0 + g * 8) = make_uint4(w[0], w[1], w[2], w[3]);
         }
       }
@@ -339,10 +326,9 @@ __global__ void __launch_bounds__(320, 1)
   __shared__ int s_first, s_last;
 
   const int warp = uniform_warp_idx(), lane = threadIdx.x & 31;
-  int idx = blockIdx.x;
-  const int kv0 = idx % p.tiles * 128;              // causal: the keys that most rows see first
-  idx /= p.tiles;
-  const int hkv = idx % p.Hkv, b = idx / p.Hkv, group = p.H / p.Hkv;
+  int kv_tile, unit;
+  span_place<false>(p.order, blockIdx.x, kv_tile, unit);      // causal: the keys that most rows see first
+  const int kv0 = kv_tile * 128, hkv = unit % p.Hkv, b = unit / p.Hkv, group = p.H / p.Hkv;
   const int off = p.Sk - p.Sq, q_tiles = p.sq_pad / 64;
   const int4* range = p.range + static_cast<long long>(b) * q_tiles;
 
@@ -496,23 +482,12 @@ __global__ void __launch_bounds__(320, 1)
       const int4 *lo4 = reinterpret_cast<const int4*>(rows + 512), *hi4 = reinterpret_cast<const int4*>(rows + 768);
       const bool masked = kv0 < r.z || kv0 + 128 > r.w;
       const int first = tile * 64 + off;                        // place of the tile's first row among the keys
-      const int side = first >= kv0 + 127 ? 1 : first + 63 <= kv0 ? -1 : 0;
+      const int side = !BIAS ? 1 : p.c.causal || first >= kv0 + 127 ? 1 : first + 63 <= kv0 ? -1 : 0;
       const uint32_t st_addr = lane_addr + C::ST_COL + (it & 1) * 64 + half * 32;
-      uint32_t s[32], dp[32], packed[16];
-      float g[32];
+      uint32_t s[32], dp[32], slip[32], packed[16];
       tmem_ld_32x32b_x32(st_addr, s);
       tmem_ld_32x32b_x32(lane_addr + C::DP_COL + (it & 1) * 64 + half * 32, dp);
       tmem_ld_wait();
-      span_scale<CAP, 32>(s, p.c);
-      if constexpr (CAP) span_slip<32>(s, p.inv_out2, g);
-      if constexpr (BIAS) span_bias<1, 32>(s, slope2, (float)(first + half * 32 - kv), side);
-#pragma unroll
-      for (int i4 = 0; i4 < 8; ++i4) {
-        const float4 l = lse4[i4];
-        const float ls[4] = {l.x, l.y, l.z, l.w};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) s[i4 * 4 + k] = __float_as_uint(fast_exp2(__uint_as_float(s[i4 * 4 + k]) - ls[k]));
-      }
       uint32_t seen = 0xffffffffu;
       if (masked) {
         seen = 0;
@@ -522,30 +497,29 @@ __global__ void __launch_bounds__(320, 1)
           seen |= (kv >= lo.x && kv < hi.x ? 1u : 0u) << (i4 * 4) | (kv >= lo.y && kv < hi.y ? 2u : 0u) << (i4 * 4) |
                   (kv >= lo.z && kv < hi.z ? 4u : 0u) << (i4 * 4) | (kv >= lo.w && kv < hi.w ? 8u : 0u) << (i4 * 4);
         }
-#pragma unroll
-        for (int k = 0; k < 32; ++k)
-          if (!(seen >> k & 1)) s[k] = 0;
+        span_mask32(s, seen, 0);         // what unseen keys hold decides nothing
+      }
+      const float away = (float)(first + half * 32 - kv), slope = side > 0 ? -slope2 : slope2, reach = CAP ? span_reach32(s) : 0.f;
+      if (BIAS && side != 0) {
+        span_score32<CAP, true>(s, p.c, SpanAdd<true, true>({slope * away, slope}, lse4), slip, reach);
+      } else {
+        span_score32<CAP, true>(s, p.c, SpanAdd<false, true>({0.f, 0.f}, lse4), slip, reach);
+        if constexpr (BIAS) span_both_sides32<1>(s, slope2, away);
       }
 #pragma unroll
-      for (int k = 0; k < 16; ++k) packed[k] = pack2<T>(__uint_as_float(s[2 * k]), __uint_as_float(s[2 * k + 1]));
+      for (int k = 0; k < 32; ++k) s[k] = __float_as_uint(fast_exp2(__uint_as_float(s[k])));
+      if (masked) span_mask32(s, seen, 0);
+      span_pack32<T>(s, packed);
       tmem_st_32x32b_x16(st_addr, packed);
 #pragma unroll
-      for (int i4 = 0; i4 < 8; ++i4) {
-        const float4 d = delta4[i4];
-        const float de[4] = {d.x, d.y, d.z, d.w};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int i = i4 * 4 + k;
-          const float w = CAP ? __uint_as_float(s[i]) * g[i] : __uint_as_float(s[i]);
-          g[i] = w * (__uint_as_float(dp[i]) - de[k]);
-        }
+      for (int k = 0; k < 32; k += 2) {
+        const float4 d = delta4[k >> 2];
+        uint64_t w = pair_at(s, k);
+        if (CAP) w = mul_f32x2(w, pair_at(slip, k));
+        set_pair(s, k, mul_f32x2(w, add_f32x2(pair_at(dp, k), k & 2 ? f32x2(d.z, d.w) : f32x2(d.x, d.y))));
       }
-      if (masked) {
-#pragma unroll
-        for (int k = 0; k < 32; ++k)
-          if (!(seen >> k & 1)) g[k] = 0.f;
-      }
-      span_pack32<T>(g, packed);
+      if (masked) span_mask32(s, seen, 0);
+      span_pack32<T>(s, packed);
       tmem_st_32x32b_x16(st_addr + 16, packed);
       tmem_st_wait();
       tc_fence_before();
@@ -559,7 +533,7 @@ __global__ void __launch_bounds__(320, 1)
     if (ok) {
       // warps 0-3 store dV, warps 4-7 dK
       T* out = reinterpret_cast<T*>(half == 0 ? p.dv : p.dk) + b * p.dkv_st[0] + kv * p.dkv_st[1] + hkv * p.dkv_st[2];
-      const float f = half == 0 ? 1.f : p.scale;
+      const float f = half == 0 ? 1.f : p.grad_scale;
 #pragma unroll 1
       for (int c = 0; c < HD / 32; ++c) {
         if (c * 32 >= p.D) break;
@@ -605,9 +579,9 @@ int launch_span_bwd(const SpanBwdMaps& m, SpanBwdParams p, cudaStream_t st) {
   if (e != cudaSuccess) return 2000 + (int)e;
   const long long q_tiles = (p.Sq + 127) / 128, kv_tiles = (p.Sk + 127) / 128;
   if (q_tiles * p.H * p.B > 0x7fffffffll || kv_tiles * p.Hkv * p.B > 0x7fffffffll) return 20;
-  p.tiles = (int)q_tiles;
+  p.order = {(int)q_tiles, p.H * p.B, rbh::span_group(static_cast<long long>(p.H) * p.B, 4ll * p.Sk * p.D * p.Hkv / p.H)};
   dq<<<(unsigned)(q_tiles * p.H * p.B), 320, SpanDqCfg<HD>::SMEM_BYTES, st>>>(m.k64, m.v64, p);
-  p.tiles = (int)kv_tiles;
+  p.order = {(int)kv_tiles, p.Hkv * p.B, rbh::span_group(static_cast<long long>(p.Hkv) * p.B, 4ll * p.Sq * p.D * (p.H / p.Hkv))};
   dkv<<<(unsigned)(kv_tiles * p.Hkv * p.B), 320, SpanDkvCfg<HD>::SMEM_BYTES, st>>>(m.q, m.k, m.v, m.dout, p);
   e = cudaGetLastError();
   return e == cudaSuccess ? 0 : 3000 + (int)e;
@@ -647,15 +621,12 @@ int rb_span_bwd(int dtype, const void* q, const void* k, const void* v, const lo
   if (Sk <= 0 || Hkv <= 0 || H % Hkv || D <= 0 || D > 128 || D % 8 || Sq > 0x7fffffff - 128) return 20;
   SpanBwdParams p{};
   p.B = B; p.H = H; p.Hkv = Hkv; p.Sq = Sq; p.Sk = Sk; p.D = D;
-  p.c.scale2 = scale * kLog2e;
-  p.c.in = cap > 0.f ? scale / cap : 0.f;
-  p.c.out2 = cap * kLog2e;
+  p.c = rbh::span_scores(scale, cap);
   p.c.slopes = slopes;
   p.c.spans = reinterpret_cast<const int2*>(spans);
   p.c.span_batch = span_batch;
   p.c.causal = causal;
-  p.scale = scale;
-  p.inv_out2 = cap > 0.f ? 1.f / p.c.out2 : 0.f;
+  p.grad_scale = cap > 0.f ? -scale : scale;
   p.q = q; p.o = o; p.dout = dout; p.lse2 = lse2;
   for (int i = 0; i < 3; ++i) { p.q_st[i] = qs[i]; p.do_st[i] = dos[i]; p.dq_st[i] = dqs[i]; p.dkv_st[i] = dkvs[i]; }
   p.sq_pad = (Sq + 63) / 64 * 64;

@@ -2,10 +2,10 @@
 // each row, 16-bit, heads of 8 to 128 numbers.
 //
 // A CTA owns two tiles of 128 query rows of one head, each with a warpgroup of its own (a thread owns a row: maximum and sum never leave it) and its
-// own S and O in tensor memory.  Tiles of 128 keys and of 128 values take turns in one ring of shared memory and serve both query tiles.  P
-// (16-bit) lies over the first half of its S, from where P V reads it as left operand, and the next S of the tile follows that product in the
-// issue order, so what a warpgroup waits for, S of its next tile, also says that P and O are at rest.  While one warpgroup waits for the tensor
-// core the other one computes.  O is rescaled only when a row's maximum moved by more than 2^8.
+// own S and O in tensor memory.  Tiles of 64 keys and of 64 values take turns in one ring of shared memory and serve both query tiles, from the last
+// to the first: the nearest keys, whose scores the distance lowers least, come first.  S of a query tile has two buffers, so that a warpgroup finds its
+// next tile's S there when it has done one: with one buffer (of 128 keys) it waited 1500 of 4300 cycles a tile for the products.  P (16-bit) lies over the
+// first half of its S, from where P V reads it as left operand; the S that follows in that buffer comes after that product in the issue order.
 //
 // Keys that no row of a tile reaches are not read: each query tile goes over the tiles from its least lo to its largest hi.  Few rows over many
 // keys would leave most SMs idle, so such calls cut the tiles of keys into `splits` parts, whose results (fp32, with their log-sum-exp) a second
@@ -13,14 +13,17 @@
 #include "span_join.cuh"
 #include "span_scores.cuh"
 
+#include <type_traits>
+
 namespace rb {
 
 struct SpanFwdParams {
   int B, H, Hkv, Sq, Sk, D;
-  int q_tiles, splits;
+  int splits;
+  SpanOrder order;   // of tiles of 256 rows and heads x parts
   SpanScores c;
   void* o;           // [B, Sq, H, D]
-  float* lse2;       // [B, H, Sq] log-sum-exp in log2 units, -inf: the row sees no key
+  float* lse2;       // [B, H, Sq] log-sum-exp in log2 units, -inf: the row sees no key (or null)
   float* part_o;     // [splits, B, Sq, H, D] (splits > 1)
   float* part_lse2;  // [splits, B, H, Sq]
   int* status;
@@ -28,36 +31,37 @@ struct SpanFwdParams {
 
 template <int HD>
 struct SpanFwdCfg {
+  static constexpr int BN = 64;                       // keys of a tile
   static constexpr int SUB = HD / 64;                 // 64-column sub-tiles of a row
-  static constexpr int SUB_BYTES = 128 * 128;         // [128 x 64] 16-bit
-  static constexpr int TILE = SUB * SUB_BYTES;
-  static constexpr int SLOTS = HD == 128 ? 5 : 9;     // K and V tiles in flight, in turn
-  static constexpr int SMEM_BYTES = (2 + SLOTS) * TILE + 1024 + 256;
-  static constexpr int S_COL = 0, O_COL = 256;        // of query tile x: + x * 128
+  static constexpr int Q_SUB = 128 * 128, Q_TILE = SUB * Q_SUB;       // 128 rows, 16-bit
+  static constexpr int KV_SUB = BN * 128, KV_TILE = SUB * KV_SUB;
+  static constexpr int STAGES = 5;                    // pairs of K and V tiles in flight
+  static constexpr int SMEM_BYTES = 2 * Q_TILE + STAGES * 2 * KV_TILE + 1024 + 256;
+  static constexpr int S_COL = 0, O_COL = 256;        // of query tile x: + x * 128; second buffer of S: + 64
+  // Two softmax warpgroups and one of which three warps work.  They share out the registers that the launch gives the block.
+  static constexpr int THREADS = 384, SOFTMAX_REGS = 224, OTHER_REGS = 56, LAUNCH_REGS = (2 * SOFTMAX_REGS + OTHER_REGS) / 3;
 };
 
 template <typename T, int HD, bool CAP, bool BIAS>
-__global__ void __launch_bounds__(320, 1)
+__global__ void __launch_bounds__(SpanFwdCfg<HD>::THREADS, 1)
     span_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
-                    const SpanFwdParams p) {
+                    const __grid_constant__ CUtensorMap to, const SpanFwdParams p) {
   using C = SpanFwdCfg<HD>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  uint8_t* sQ = smem;                                  // [2][TILE]
-  uint8_t* sKV = sQ + 2 * C::TILE;                     // [SLOTS][TILE]: K0 V0 K1 V1 ...
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sKV + C::SLOTS * C::TILE);
-  uint64_t *q_full = bars, *full = bars + 1, *empty = full + C::SLOTS, *s_full = empty + C::SLOTS, *p_ready = s_full + 2, *o_done = p_ready + 2;
-  uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(o_done + 2);
+  uint8_t* sQ = smem;                                  // [2][Q_TILE], at the end O
+  uint8_t* sKV = sQ + 2 * C::Q_TILE;                   // [STAGES][2][KV_TILE]: {K0, K1}, {V0, K2}, {V1, K3}, ...
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sKV + C::STAGES * 2 * C::KV_TILE);
+  // s_full, p_ready: [query tile][buffer]; o_done: [query tile], after the last product with V; o_last: [query tile], after the one before
+  uint64_t *q_full = bars, *full = bars + 1, *empty = full + C::STAGES, *s_full = empty + C::STAGES, *p_ready = s_full + 4, *o_done = p_ready + 4, *o_last = o_done + 2;
+  uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(o_last + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_ptr + 1);
   __shared__ int4 s_range[8];
 
   const int warp = uniform_warp_idx(), lane = threadIdx.x & 31;
-  int idx = blockIdx.x;
-  const int q_tile = p.q_tiles - 1 - idx % p.q_tiles;  // causal: the longest first
-  idx /= p.q_tiles;
-  const int sp = idx % p.splits;
-  idx /= p.splits;
-  const int h = idx % p.H, b = idx / p.H;
+  int q_tile, unit;
+  span_place<true>(p.order, blockIdx.x, q_tile, unit);
+  const int sp = unit % p.splits, h = unit / p.splits % p.H, b = unit / p.splits / p.H;
   const int hkv = h / (p.H / p.Hkv);
   const int q0 = q_tile * 256, off = p.Sk - p.Sq;
 
@@ -65,16 +69,17 @@ __global__ void __launch_bounds__(320, 1)
     prefetch_tensormap(&tq);
     prefetch_tensormap(&tk);
     prefetch_tensormap(&tv);
+    prefetch_tensormap(&to);
     mbar_init(smem_u32(q_full), 1);
-    for (int s = 0; s < C::SLOTS; ++s) {
+    for (int s = 0; s < C::STAGES; ++s) {
       mbar_init(smem_u32(&full[s]), 1);
-      mbar_init(smem_u32(&empty[s]), 1);
+      mbar_init(smem_u32(&empty[s]), 2);        // both query tiles' products
     }
-    for (int x = 0; x < 2; ++x) {
-      mbar_init(smem_u32(&s_full[x]), 1);
-      mbar_init(smem_u32(&p_ready[x]), 128);
-      mbar_init(smem_u32(&o_done[x]), 1);
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(smem_u32(&s_full[i]), 1);
+      mbar_init(smem_u32(&p_ready[i]), 128);
     }
+    for (int x = 0; x < 4; ++x) mbar_init(smem_u32(&o_done[x]), 1);      // o_last too
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -99,8 +104,8 @@ __global__ void __launch_bounds__(320, 1)
 #pragma unroll
   for (int x = 0; x < 2; ++x) {
     const int4 r = span_range_join(span_range_join(s_range[4 * x], s_range[4 * x + 1]), span_range_join(s_range[4 * x + 2], s_range[4 * x + 3]));
-    first[x] = r.x < r.y ? r.x / 128 : 0;
-    last[x] = r.x < r.y ? (r.y + 127) / 128 : 0;
+    first[x] = r.x < r.y ? r.x / C::BN : 0;
+    last[x] = r.x < r.y ? (r.y + C::BN - 1) / C::BN : 0;
     lo_all[x] = r.z;
     hi_all[x] = r.w;
   }
@@ -110,197 +115,295 @@ __global__ void __launch_bounds__(320, 1)
     j0 = a && c ? min(first[0], first[1]) : a ? first[0] : first[1];
     j1 = max(last[0], last[1]);
     const int per = (j1 - j0 + p.splits - 1) / p.splits;
-    const int from = j0 + sp * per, to = min(j1, from + per);
+    const int from = j0 + sp * per, to_ = min(j1, from + per);
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
       first[x] = max(first[x], from);
-      last[x] = max(first[x], min(last[x], to));
+      last[x] = max(first[x], min(last[x], to_));
     }
     j0 = from;
-    j1 = max(from, to);
+    j1 = max(from, to_);
   }
   const int n = j1 - j0;
-  auto active = [&](int x, int j) { return first[x] <= j && j < last[x]; };
 
-  if (warp == 8) {
-    // ------------------------------ TMA producer ------------------------------
-    if (lane == 0 && n > 0) {
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::OTHER_REGS));
+    if (warp == 8 && lane == 0 && n > 0) {
+      // ------------------------------ TMA producer ------------------------------
       const bool two = q0 + 128 < p.Sq;
-      mbar_arrive_expect_tx(smem_u32(q_full), (two ? 2 : 1) * C::TILE);
+      mbar_arrive_expect_tx(smem_u32(q_full), (two ? 2 : 1) * C::Q_TILE);
 #pragma unroll
       for (int s = 0; s < C::SUB; ++s) {
-        tma_load_4d(smem_u32(sQ + s * C::SUB_BYTES), &tq, smem_u32(q_full), s * 64, q0, h, b);
-        if (two) tma_load_4d(smem_u32(sQ + C::TILE + s * C::SUB_BYTES), &tq, smem_u32(q_full), s * 64, q0 + 128, h, b);
+        tma_load_4d(smem_u32(sQ + s * C::Q_SUB), &tq, smem_u32(q_full), s * 64, q0, h, b);
+        if (two) tma_load_4d(smem_u32(sQ + C::Q_TILE + s * C::Q_SUB), &tq, smem_u32(q_full), s * 64, q0 + 128, h, b);
       }
       bool ok = true;
-      int slot = 0;
+      int st = 0;
       uint32_t ph = 0;
-      for (int i = 0; i < 2 * n; ++i) {
-        ok = mbar_wait(smem_u32(&empty[slot]), ph ^ 1, abort_flag, p.status, RB_ERR_TIMEOUT_EMPTY);
-        if (!ok) break;
-        const uint32_t bar = smem_u32(&full[slot]);
-        mbar_arrive_expect_tx(bar, C::TILE);
+      // two tiles (b: one of keys behind the last: none)
+      auto bring = [&](const CUtensorMap* map_a, int a, int b_) {
+        ok = mbar_wait(smem_u32(&empty[st]), ph ^ 1, abort_flag, p.status, RB_ERR_TIMEOUT_EMPTY);
+        if (!ok) return;
+        const uint32_t bar = smem_u32(&full[st]), dst = smem_u32(sKV + st * 2 * C::KV_TILE);
+        mbar_arrive_expect_tx(bar, (b_ >= j0 ? 2 : 1) * C::KV_TILE);
 #pragma unroll
-        for (int s = 0; s < C::SUB; ++s)
-          tma_load_4d(smem_u32(sKV + slot * C::TILE + s * C::SUB_BYTES), i & 1 ? &tv : &tk, bar, s * 64, (j0 + (i >> 1)) * 128, hkv, b);
-        if (++slot == C::SLOTS) { slot = 0; ph ^= 1; }
-      }
+        for (int s = 0; s < C::SUB; ++s) {
+          tma_load_4d(dst + s * C::KV_SUB, map_a, bar, s * 64, a * C::BN, hkv, b);
+          if (b_ >= j0) tma_load_4d(dst + C::KV_TILE + s * C::KV_SUB, &tk, bar, s * 64, b_ * C::BN, hkv, b);
+        }
+        if (++st == C::STAGES) { st = 0; ph ^= 1; }
+      };
+      bring(&tk, j1 - 1, j1 - 2);
+      for (int j = j1 - 1; j >= j0 && ok; --j) bring(&tv, j, j - 2);
       if (!ok)
         for (int i = 0; i < 64; ++i) __nanosleep(10000);      // copies in flight land before the CTA's memory goes
-    }
-  } else if (warp == 9) {
-    // ------------------------------ MMA issuer --------------------------------
-    if (n > 0) {
-      constexpr uint32_t idesc_s = make_idesc(UmmaFormat<T>::value, 0, 0, 128, 128);
+    } else if ((warp == 9 || warp == 10) && n > 0) {
+      // ------------------------------ MMA issuers -------------------------------
+      // One warp per query tile: what a warp does between its products (waits and commits, some 100 cycles each) takes as long as they do.
+      const int x = warp - 9;
+      const int begin = x ? first[1] : first[0], end = x ? last[1] : last[0];
+      constexpr uint32_t idesc_s = make_idesc(UmmaFormat<T>::value, 0, 0, 128, C::BN);
       constexpr uint32_t idesc_o = make_idesc(UmmaFormat<T>::value, 0, 1, 128, HD);
-      auto issue_s = [&](int x, int slot) {
-        const uint64_t qd = make_smem_desc_sw128(smem_u32(sQ + x * C::TILE), 16, 1024);
-        const uint64_t kd = make_smem_desc_sw128(smem_u32(sKV + slot * C::TILE), 16, 1024);
+      const uint32_t s_tmem = tmem_base + C::S_COL + x * 128, o_tmem = tmem_base + C::O_COL + x * 128;
+      const uint64_t qd = make_smem_desc_sw128(smem_u32(sQ + x * C::Q_TILE), 16, 1024);
+      int st = 0;
+      uint32_t ph = 0;
+      auto issue_s = [&](int j, int at) {                     // K(j) in half `at` of the stage
+        if (j < begin || j >= end) return;
+        const int buf = (end - 1 - j) & 1;
+        const uint64_t kd = make_smem_desc_sw128(smem_u32(sKV + (2 * st + at) * C::KV_TILE), 16, 1024);
 #pragma unroll
         for (int s = 0; s < C::SUB; ++s)
-          umma_f16_w4<2, 2>(tmem_base + C::S_COL + x * 128, qd + s * (C::SUB_BYTES >> 4), kd + s * (C::SUB_BYTES >> 4), idesc_s, s != 0);
-        umma_commit_w(smem_u32(&s_full[x]));
+          umma_f16_w4<2, 2>(s_tmem + buf * 64, qd + s * (C::Q_SUB >> 4), kd + s * (C::KV_SUB >> 4), idesc_s, s != 0);
+        umma_commit_w(smem_u32(&s_full[2 * x + buf]));
+      };
+      auto leave = [&]() {
+        umma_commit_w(smem_u32(&empty[st]));
+        if (++st == C::STAGES) { st = 0; ph ^= 1; }
       };
       bool ok = mbar_wait(smem_u32(q_full), 0, abort_flag, p.status, RB_ERR_TIMEOUT_FULL);
       if (ok) ok = mbar_wait(smem_u32(&full[0]), 0, abort_flag, p.status, RB_ERR_TIMEOUT_FULL);
       if (ok) {
         tc_fence_after();
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-          if (active(x, j0)) issue_s(x, 0);
-        umma_commit_w(smem_u32(&empty[0]));
+        issue_s(j1 - 1, 0);
+        issue_s(j1 - 2, 1);
+        leave();
       }
-      int slot = 1;                    // of V(j); K(j + 1) stands in the next one
-      uint32_t ph = 0, p_ph[2] = {0, 0};
-      for (int j = j0; j < j1 && ok; ++j) {
-        const int slot_k = slot + 1 == C::SLOTS ? 0 : slot + 1;
-        const uint32_t ph_k = slot + 1 == C::SLOTS ? ph ^ 1 : ph;
-        const bool more = j + 1 < j1;
-        bool k_here = false;
-        ok = mbar_wait(smem_u32(&full[slot]), ph, abort_flag, p.status, RB_ERR_TIMEOUT_FULL);
+      for (int j = j1 - 1; j >= j0 && ok; --j) {
+        ok = mbar_wait(smem_u32(&full[st]), ph, abort_flag, p.status, RB_ERR_TIMEOUT_FULL);
         if (!ok) break;
-        const uint64_t vd = make_smem_desc_sw128(smem_u32(sKV + slot * C::TILE), C::SUB_BYTES, 1024);
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          if (ok && active(x, j)) {
-            ok = mbar_wait(smem_u32(&p_ready[x]), p_ph[x], abort_flag, p.status, RB_ERR_TIMEOUT_FLAG);
-            if (ok) {
-              p_ph[x] ^= 1;
-              tc_fence_after();
-#pragma unroll
-              for (int s = 0; s < 2; ++s)
-                umma_f16_ts_w4<8, 128>(tmem_base + C::O_COL + x * 128, tmem_base + C::S_COL + x * 128 + s * 32, vd + s * 512, idesc_o,
-                                       (j > first[x] || s != 0) ? 1u : 0u);
-              if (j + 1 == last[x]) umma_commit_w(smem_u32(&o_done[x]));
-            }
-          }
-          if (ok && more && active(x, j + 1)) {
-            if (!k_here) ok = mbar_wait(smem_u32(&full[slot_k]), ph_k, abort_flag, p.status, RB_ERR_TIMEOUT_FULL);
-            if (ok) {
-              k_here = true;
-              tc_fence_after();
-              issue_s(x, slot_k);
-            }
-          }
-        }
-        if (!ok) break;
-        umma_commit_w(smem_u32(&empty[slot]));
-        if (more) {
-          if (!k_here) ok = mbar_wait(smem_u32(&full[slot_k]), ph_k, abort_flag, p.status, RB_ERR_TIMEOUT_FULL);   // a tile that neither reaches
+        if (j >= begin && j < end) {
+          const int i = end - 1 - j, buf = i & 1;
+          ok = mbar_wait(smem_u32(&p_ready[2 * x + buf]), (i >> 1) & 1, abort_flag, p.status, RB_ERR_TIMEOUT_FLAG);
           if (!ok) break;
-          umma_commit_w(smem_u32(&empty[slot_k]));
+          tc_fence_after();
+          umma_f16_ts_w4<8, 128>(o_tmem, s_tmem + buf * 64, make_smem_desc_sw128(smem_u32(sKV + 2 * st * C::KV_TILE), C::KV_SUB, 1024), idesc_o, i != 0);
+          if (j <= begin + 1) umma_commit_w(smem_u32(j == begin ? &o_done[x] : &o_last[x]));
+        } else {
+          tc_fence_after();
         }
-        slot = slot_k + 1 == C::SLOTS ? 0 : slot_k + 1;
-        ph = slot_k + 1 == C::SLOTS ? ph_k ^ 1 : ph_k;
+        issue_s(j - 2, 1);
+        leave();
       }
     }
   } else {
     // ------------------------------ softmax warpgroups ------------------------
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::SOFTMAX_REGS));
     const int x = warp >> 2, t = threadIdx.x & 127;
     const int row0 = q0 + x * 128, row = row0 + t;
     const uint32_t lane_addr = tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-    const uint32_t s_addr = lane_addr + C::S_COL + x * 128, o_addr = lane_addr + C::O_COL + x * 128;
+    const uint32_t o_addr = lane_addr + C::O_COL + x * 128;
     const int begin = x ? first[1] : first[0], end = x ? last[1] : last[0];
     const int lo_max = x ? lo_all[1] : lo_all[0], hi_min = x ? hi_all[1] : hi_all[0];
     const float slope2 = BIAS ? p.c.slopes[h] * kLog2e : 0.f;
-    float m = -INFINITY, l = 0.f;                 // maximum that P is relative to, and sum
-    bool ok = true;
-    uint32_t ph = 0;
-    for (int j = begin; j < end; ++j, ph ^= 1) {
-      ok = mbar_wait(smem_u32(&s_full[x]), ph, abort_flag, p.status, RB_ERR_TIMEOUT_TMEM_FULL);
+    // Weights are relative to `ref`, which follows the row's maximum only when that may be far away: a tile's weights are made in one pass over its
+    // scores, without their maximum (the second half's scores, on the FMA pipe, between the first one's exponentials, on the special-function
+    // pipe).  Where the largest product says that the reference may be no good, the tile is done again in two passes.
+    // How far from its reference a weight may be: fp16 ones go up to 2^16, and small ones lose bits below 2^-14; bf16 has the range of fp32.
+    // (Not all of it: what a value of 2^90 times a weight of 2^30 is still has to be a number.)  LEAST: of a first tile's sum.
+    constexpr float UP = UmmaFormat<T>::value == 1 ? 30.f : 15.f, LEAST = UmmaFormat<T>::value == 1 ? 1.f / (1 << 30) : 1.f / (1 << 8);
+    float ref = 0.f, l = 0.f;
+    bool fresh = true, ok = true;                       // fresh: the row has seen no key yet
+    bool flat = false, slow = false;                    // what the last tile needed: the general tanh, the two passes
+    for (int i = 0; i < end - begin; ++i) {
+      const int buf = i & 1;
+      ok = mbar_wait(smem_u32(&s_full[2 * x + buf]), (i >> 1) & 1, abort_flag, p.status, RB_ERR_TIMEOUT_TMEM_FULL);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();
-      const int kv0 = j * 128;
-      uint32_t s[4][32];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(s_addr + c * 32, s[c]);
-      tmem_ld_wait();
-      const bool masked = kv0 < lo_max || kv0 + 128 > hi_min;
-      const int side = row0 + off >= kv0 + 127 ? 1 : row0 + 127 + off <= kv0 ? -1 : 0;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        span_scale<CAP, 32>(s[c], p.c);
-        if constexpr (BIAS) span_bias<-1, 32>(s[c], slope2, (float)(row + off - kv0 - c * 32), side);
-      }
-      if (masked) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const uint32_t seen = span_bits(span.x - kv0 - c * 32, span.y - kv0 - c * 32);
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (!(seen >> i & 1)) s[c][i] = 0xff800000u;
+      const uint32_t s_addr = lane_addr + C::S_COL + x * 128 + buf * 64;
+      const int kv0 = (end - 1 - i) * C::BN;
+      const bool masked = kv0 < lo_max || kv0 + C::BN > hi_min;
+      // where all distances that count have one sign the bias is a ramp
+      const int side = !BIAS ? 1 : p.c.causal || row0 + off >= kv0 + C::BN - 1 ? 1 : row0 + 127 + off <= kv0 ? -1 : 0;
+      const float slope = side > 0 ? slope2 : -slope2;
+      const int away = row + off - kv0;                  // distance of the tile's first key
+      // chunk c of 32 scores, plus `base`, what is unseen -inf; whether it has something to see; the largest product
+      float reach = 0.f;
+      auto scores = [&](int c, float base, uint32_t* s) -> bool {
+        uint32_t seen = 0xffffffffu;
+        bool part = false;
+        if (masked) {
+          seen = span_bits(span.x - kv0 - c * 32, span.y - kv0 - c * 32);
+          if (__all_sync(0xffffffffu, seen == 0)) return false;
+          part = !__all_sync(0xffffffffu, seen == 0xffffffffu);
         }
-      }
-      float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-#pragma unroll
-        for (int i = 0; i < 32; i += 2)
-          mx4[(i >> 1) & 3] = fmaxf(fmaxf(mx4[(i >> 1) & 3], __uint_as_float(s[c][i])), __uint_as_float(s[c][i + 1]));
-      const float m_new = fmaxf(m, fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])));
-      const bool need = m_new > m + 8.0f;         // also the first time that the row sees a key
-      if (__any_sync(0xffffffffu, need)) {        // tensor memory is accessed by whole warps
-        float alpha = 1.0f;
-        if (need) {
-          alpha = m == -INFINITY ? 0.0f : fast_exp2(m - m_new);
-          m = m_new;
-          l *= alpha;
+        tmem_ld_32x32b_x32(s_addr + c * 32, s);
+        tmem_ld_wait();
+        if (part) span_mask32(s, seen, 0);               // what unseen keys hold decides nothing
+        reach = fmaxf(reach, span_reach32(s));
+        if (BIAS && side != 0) {
+          span_score32<CAP, false>(s, p.c, SpanAdd<true, false>({fmaf(-slope, (float)(away - c * 32), base), slope}, nullptr), nullptr, reach);
+        } else {
+          span_score32<CAP, false>(s, p.c, SpanAdd<false, false>({base, 0.f}, nullptr), nullptr, reach);
+          if constexpr (BIAS) span_both_sides32<-1>(s, slope2, (float)(away - c * 32));
         }
-        if (j > begin) {
-#pragma unroll 1
-          for (int c = 0; c < HD / 16; ++c) {
-            uint32_t r[16];
-            tmem_ld_32x32b_x16(o_addr + c * 16, r);
-            tmem_ld_wait();
+        if (part) span_mask32(s, seen, 0xff800000u);
+        return true;
+      };
+      // weights of a chunk of scores relative to ref
+      auto weights = [&](const uint32_t* s, uint32_t* packed) -> float {
+        uint64_t l2[2] = {0, 0};
 #pragma unroll
-            for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * alpha);
-            tmem_st_32x32b_x16(o_addr + c * 16, r);
+        for (int k = 0; k < 16; ++k) {
+          const float p0 = fast_exp2(__uint_as_float(s[2 * k])), p1 = fast_exp2(__uint_as_float(s[2 * k + 1]));
+          l2[k & 1] = add_f32x2(l2[k & 1], f32x2(p0, p1));
+          packed[k] = pack2<T>(p0, p1);
+        }
+        const float2 la = f32x2_get(l2[0]), lb = f32x2_get(l2[1]);
+        return (la.x + la.y) + (lb.x + lb.y);
+      };
+      const bool sees = span.x < min(kv0 + C::BN, span.y) && span.y > max(kv0, span.x);
+      bool done = false;
+      if (!slow) {
+        uint32_t packed[2][16];
+        float sum = 0.f;
+        bool quick = !masked && side != 0 && !(CAP && flat);
+        if (quick) {
+          const SpanTanh f(p.c, p.c.out2);
+          const uint64_t k = both(p.c.scale2);
+          float far[4] = {0.f, 0.f, 0.f, 0.f};
+          auto score = [&](uint32_t* s, int i, auto& add) {
+            far[i & 2] = fmaxf(far[i & 2], fabsf(__uint_as_float(s[i])));
+            far[(i & 2) + 1] = fmaxf(far[(i & 2) + 1], fabsf(__uint_as_float(s[i + 1])));
+            if constexpr (CAP) {
+              const uint64_t x2 = pair_at(s, i);
+              set_pair(s, i, fma_f32x2(x2, f.r(x2), add.next(i)));
+            } else {
+              set_pair(s, i, fma_f32x2(pair_at(s, i), k, add.next(i)));
+            }
+          };
+          // scores LAG pairs ahead of the weights: the FMA pipe and the special-function pipe work at the same time all along
+          constexpr int LAG = 4;
+          uint32_t s[64];
+          tmem_ld_32x32b_x32(s_addr, s);
+          tmem_ld_32x32b_x32(s_addr + 32, s + 32);
+          tmem_ld_wait();
+          SpanAdd<BIAS, false> add({BIAS ? fmaf(-slope, (float)away, -ref) : -ref, slope}, nullptr);
+#pragma unroll
+          for (int g = 0; g < LAG; ++g) score(s, 2 * g, add);
+          uint64_t l2[2] = {0, 0};
+#pragma unroll
+          for (int g = 0; g < 32; ++g) {
+            // the ramp begins anew half-way
+            if (BIAS && g + LAG == 16) add = SpanAdd<BIAS, false>({fmaf(-slope, (float)(away - 32), -ref), slope}, nullptr);
+            const float p0 = fast_exp2(__uint_as_float(s[2 * g])), p1 = fast_exp2(__uint_as_float(s[2 * g + 1]));
+            if (g + LAG < 32) score(s, 2 * (g + LAG), add);
+            l2[g & 1] = add_f32x2(l2[g & 1], f32x2(p0, p1));
+            packed[g >> 4][g & 15] = pack2<T>(p0, p1);
+          }
+          const float2 la = f32x2_get(l2[0]), lb = f32x2_get(l2[1]);
+          sum = (la.x + la.y) + (lb.x + lb.y);
+          reach = fmaxf(fmaxf(far[0], far[1]), fmaxf(far[2], far[3]));
+          if constexpr (CAP) {
+            flat = __any_sync(0xffffffffu, !(reach <= p.c.near));
+            quick = !flat;
           }
         }
-      }
-      const float neg = m == -INFINITY ? 0.f : -m;
-      const uint64_t neg2 = f32x2(neg, neg);
-      uint64_t l2[2] = {0, 0};
+        if (!quick) {
+          // chunk by chunk: some have nothing to see, some all, some large products
+          sum = reach = 0.f;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t packed[16];
+          for (int c = 0; c < 2; ++c) {
+            uint32_t s[32];
+            if (scores(c, -ref, s)) {
+              sum += weights(s, packed[c]);
+            } else {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float2 y = f32x2_get(add_f32x2(f32x2(__uint_as_float(s[c][2 * i]), __uint_as_float(s[c][2 * i + 1])), neg2));
-          const float p0 = fast_exp2(y.x), p1 = fast_exp2(y.y);
-          l2[i & 1] = add_f32x2(l2[i & 1], f32x2(p0, p1));
-          packed[i] = pack2<T>(p0, p1);
+              for (int k = 0; k < 16; ++k) packed[c][k] = 0;
+            }
+          }
+          if (CAP && !masked) flat = __any_sync(0xffffffffu, !(reach <= p.c.near));
         }
-        tmem_st_32x32b_x16(s_addr + c * 16, packed);
+        // no score of the row is above this: the cap and the largest product bound it
+        float most = reach * fabsf(p.c.scale2);
+        if (CAP) most = fminf(most, p.c.out2);
+        if (BIAS && slope2 < 0.f) most = fmaf(-slope2, (float)max(abs(away), abs(away - C::BN + 1)), most);
+        done = __all_sync(0xffffffffu, most - ref <= UP && (!fresh || !sees || sum >= LEAST));
+        if (done) {
+          l += sum;
+          fresh = fresh && !sees;
+          tmem_st_32x32b_x16(s_addr, packed[0]);
+          tmem_st_32x32b_x16(s_addr + 16, packed[1]);
+        }
       }
-      const float2 la = f32x2_get(l2[0]), lb = f32x2_get(l2[1]);
-      l += (la.x + la.y) + (lb.x + lb.y);
+      if (!done) {
+        float mx = -INFINITY;
+        reach = 0.f;
+#pragma unroll 1
+        for (int c = 0; c < 2; ++c) {
+          uint32_t s[32];
+          if (!scores(c, 0.f, s)) continue;
+#pragma unroll
+          for (int k = 0; k < 32; ++k) mx = fmaxf(mx, __uint_as_float(s[k]));
+        }
+        // a maximum that goes on rising is looked for at once in the next tile
+        slow = !__all_sync(0xffffffffu, fresh || mx <= ref + UP);
+        const bool need = mx > ref + UP || (fresh && mx > -INFINITY);
+        if (__any_sync(0xffffffffu, need)) {               // tensor memory is accessed by whole warps
+          const float alpha = !need ? 1.f : fresh ? 0.f : fast_exp2(ref - mx);
+          if (need) ref = mx;
+          l *= alpha;
+          if (i > 0) {
+            // O is at rest once the last tile's product has retired: the next tile's S comes after it
+            ok = i + 1 < end - begin
+                     ? mbar_wait(smem_u32(&s_full[2 * x + (buf ^ 1)]), ((i + 1) >> 1) & 1, abort_flag, p.status, RB_ERR_TIMEOUT_TMEM_EMPTY)
+                     : mbar_wait(smem_u32(&o_last[x]), 0, abort_flag, p.status, RB_ERR_TIMEOUT_TMEM_EMPTY);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < HD / 16; ++c) {
+              uint32_t r[16];
+              tmem_ld_32x32b_x16(o_addr + c * 16, r);
+              tmem_ld_wait();
+#pragma unroll
+              for (int k = 0; k < 16; ++k) r[k] = __float_as_uint(__uint_as_float(r[k]) * alpha);
+              tmem_st_32x32b_x16(o_addr + c * 16, r);
+            }
+          }
+        }
+        fresh = fresh && mx == -INFINITY;
+        // P of chunk c goes over what chunk 0 was read from
+#pragma unroll 1
+        for (int c = 0; c < 2; ++c) {
+          uint32_t s[32], packed[16];
+          if (scores(c, -ref, s)) {
+            l += weights(s, packed);
+          } else {
+#pragma unroll
+            for (int k = 0; k < 16; ++k) packed[k] = 0;
+          }
+          tmem_st_32x32b_x16(s_addr + c * 16, packed);
+        }
+      }
       tmem_st_wait();
       tc_fence_before();
-      mbar_arrive(smem_u32(&p_ready[x]));
+      mbar_arrive(smem_u32(&p_ready[2 * x + buf]));
     }
-    if (ok && begin < end) {
+    const int tiles = end - begin;
+    const bool staged = p.splits == 1 && tiles > 0;
+    if (ok && tiles > 0) {
       ok = mbar_wait(smem_u32(&o_done[x]), 0, abort_flag, p.status, RB_ERR_TIMEOUT_TMEM_EMPTY);
       ok = __all_sync(0xffffffffu, ok);
       tc_fence_after();
@@ -309,39 +412,56 @@ __global__ void __launch_bounds__(320, 1)
       const float inv = l > 0.f ? 1.0f / l : l != l ? l : 0.f;
       const long long at = ((static_cast<long long>(b) * p.Sq + row) * p.H + h) * p.D;
       const long long part = static_cast<long long>(sp) * p.B * p.H * p.Sq;
+      // O through shared memory, in the place of Q, and from there to memory in whole rows: a thread's row of its own stores, 16 bytes of a line each, took
+      // 6000 to 10000 cycles.  Tiles without keys (whose Q may be on its way) and the parts' sums are stored row by row.
+      uint8_t* stage = sQ + x * C::Q_TILE + t * 128;
 #pragma unroll 1
       for (int c = 0; c < HD / 32; ++c) {
         if (c * 32 >= p.D) break;
         uint32_t r[32];
-        if (begin < end) {
+        if (tiles > 0) {
           tmem_ld_32x32b_x32(o_addr + c * 32, r);
           tmem_ld_wait();
         } else {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) r[i] = 0;
+          for (int k = 0; k < 32; ++k) r[k] = 0;
         }
-        if (row >= p.Sq) continue;
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          if (c * 32 + g * 8 >= p.D) break;
           float f[8];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) f[i] = l == 0.f ? 0.f : __uint_as_float(r[g * 8 + i]) * inv;
-          if (p.splits == 1) {
-            *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.o) + at + c * 32 + g * 8) =
-                make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
-          } else {
-            float4* to = reinterpret_cast<float4*>(p.part_o + part * p.D + at + c * 32 + g * 8);
-            to[0] = make_float4(f[0], f[1], f[2], f[3]);
-            to[1] = make_float4(f[4], f[5], f[6], f[7]);
+          for (int k = 0; k < 8; ++k) f[k] = l == 0.f ? 0.f : __uint_as_float(r[g * 8 + k]) * inv;
+          const uint4 v = make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
+          const int d = c * 32 + g * 8;
+          if (staged) {
+            *reinterpret_cast<uint4*>(stage + (d >> 6) * C::Q_SUB + ((((d >> 3) & 7) ^ (t & 7)) << 4)) = v;
+          } else if (row < p.Sq && d < p.D) {
+            if (p.splits == 1) {
+              *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.o) + at + d) = v;
+            } else {
+              float4* dst = reinterpret_cast<float4*>(p.part_o + part * p.D + at + d);
+              dst[0] = make_float4(f[0], f[1], f[2], f[3]);
+              dst[1] = make_float4(f[4], f[5], f[6], f[7]);
+            }
           }
         }
       }
       if (row < p.Sq) {
         const long long r = (static_cast<long long>(b) * p.H + h) * p.Sq + row;
-        const float v = l == 0.f ? -INFINITY : m + log2f(l);
-        if (p.splits == 1) p.lse2[r] = v;
-        else p.part_lse2[part + r] = v;
+        const float v = l == 0.f ? -INFINITY : ref + log2f(l);
+        if (p.splits > 1) p.part_lse2[part + r] = v;
+        else if (p.lse2 != nullptr) p.lse2[r] = v;
+      }
+    }
+    if (staged) {
+      fence_proxy_async_smem();
+      asm volatile("bar.sync %0, 128;" ::"r"(1 + x) : "memory");      // the warpgroup, also where a wait ran out
+      if (t == 0 && ok) {
+#pragma unroll
+        for (int s = 0; s < C::SUB; ++s)
+          if (s * 64 < p.D) tma_store_4d(&to, smem_u32(sQ + x * C::Q_TILE + s * C::Q_SUB), s * 64, row0, h, b);
+        tma_store_commit();
+        tma_store_wait_read<0>();
       }
     }
   }
@@ -355,11 +475,17 @@ __global__ void __launch_bounds__(320, 1)
 }
 
 template <typename T, int HD, bool CAP, bool BIAS>
-int launch_span_fwd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const SpanFwdParams& p, unsigned grid, cudaStream_t st) {
+int launch_span_fwd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& to, const SpanFwdParams& p, unsigned grid,
+                    cudaStream_t st) {
+  using C = SpanFwdCfg<HD>;
   auto kern = span_fwd_kernel<T, HD, CAP, BIAS>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SpanFwdCfg<HD>::SMEM_BYTES);
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM_BYTES);
   if (e != cudaSuccess) return 2000 + (int)e;
-  kern<<<grid, 320, SpanFwdCfg<HD>::SMEM_BYTES, st>>>(tq, tk, tv, p);
+  cudaFuncAttributes fa;
+  e = cudaFuncGetAttributes(&fa, kern);
+  if (e != cudaSuccess) return 2000 + (int)e;
+  if (fa.numRegs < C::LAUNCH_REGS) return 21;      // the warpgroups would wait for registers that the block does not have
+  kern<<<grid, C::THREADS, C::SMEM_BYTES, st>>>(tq, tk, tv, to, p);
   e = cudaGetLastError();
   return e == cudaSuccess ? 0 : 3000 + (int)e;
 }
@@ -367,19 +493,22 @@ int launch_span_fwd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensor
 template <typename T>
 int span_fwd(int dtype, const void* q, const void* k, const void* v, const long long* qs, const long long* ks, const long long* vs, SpanFwdParams p,
              bool cap, cudaStream_t st) {
-  CUtensorMap tq, tk, tv;
+  CUtensorMap tq, tk, tv, to;
+  const long long os[3] = {static_cast<long long>(p.Sq) * p.H * p.D, static_cast<long long>(p.H) * p.D, p.D};
   int rc = rbh::span_map(&tq, dtype, q, qs, p.B, p.Sq, p.H, p.D, 128);
-  if (!rc) rc = rbh::span_map(&tk, dtype, k, ks, p.B, p.Sk, p.Hkv, p.D, 128);
-  if (!rc) rc = rbh::span_map(&tv, dtype, v, vs, p.B, p.Sk, p.Hkv, p.D, 128);
+  if (!rc) rc = rbh::span_map(&tk, dtype, k, ks, p.B, p.Sk, p.Hkv, p.D, 64);
+  if (!rc) rc = rbh::span_map(&tv, dtype, v, vs, p.B, p.Sk, p.Hkv, p.D, 64);
+  if (!rc) rc = rbh::span_map(&to, dtype, p.o, os, p.B, p.Sq, p.H, p.D, 128);
   if (rc) return 1000 + rc;
-  const long long grid = static_cast<long long>(p.q_tiles) * p.splits * p.H * p.B;
+  const long long units = static_cast<long long>(p.splits) * p.H * p.B, grid = units * ((p.Sq + 255) / 256);
   if (grid > 0x7fffffffll) return 20;
+  p.order = {(p.Sq + 255) / 256, (int)units, rbh::span_group(units, 4ll * p.Sk * p.D * p.Hkv / (p.splits * p.H) + 1)};
   const bool bias = p.c.slopes != nullptr;
-#define RB_SPAN(HD_)                                                                                      \
-  (cap ? bias ? launch_span_fwd<T, HD_, true, true>(tq, tk, tv, p, (unsigned)grid, st)                    \
-              : launch_span_fwd<T, HD_, true, false>(tq, tk, tv, p, (unsigned)grid, st)                   \
-       : bias ? launch_span_fwd<T, HD_, false, true>(tq, tk, tv, p, (unsigned)grid, st)                   \
-              : launch_span_fwd<T, HD_, false, false>(tq, tk, tv, p, (unsigned)grid, st))
+#define RB_SPAN(HD_)                                                                                          \
+  (cap ? bias ? launch_span_fwd<T, HD_, true, true>(tq, tk, tv, to, p, (unsigned)grid, st)                    \
+              : launch_span_fwd<T, HD_, true, false>(tq, tk, tv, to, p, (unsigned)grid, st)                   \
+       : bias ? launch_span_fwd<T, HD_, false, true>(tq, tk, tv, to, p, (unsigned)grid, st)                   \
+              : launch_span_fwd<T, HD_, false, false>(tq, tk, tv, to, p, (unsigned)grid, st))
   rc = p.D <= 64 ? RB_SPAN(64) : RB_SPAN(128);
 #undef RB_SPAN
   if (rc || p.splits == 1) return rc;
@@ -410,11 +539,8 @@ int rb_span_fwd(int dtype, const void* q, const void* k, const void* v, const lo
   if (Sk <= 0 || Hkv <= 0 || H % Hkv || D <= 0 || D > 128 || D % 8 || splits < 1 || (splits > 1 && (!part_o || !part_lse2))) return 20;
   SpanFwdParams p{};
   p.B = B; p.H = H; p.Hkv = Hkv; p.Sq = Sq; p.Sk = Sk; p.D = D;
-  p.q_tiles = (Sq + 255) / 256;
   p.splits = splits;
-  p.c.scale2 = scale * kLog2e;
-  p.c.in = cap > 0.f ? scale / cap : 0.f;
-  p.c.out2 = cap * kLog2e;
+  p.c = rbh::span_scores(scale, cap);
   p.c.slopes = slopes;
   p.c.spans = reinterpret_cast<const int2*>(spans);
   p.c.span_batch = span_batch;

@@ -68,6 +68,16 @@ __device__ __forceinline__ void span_store4(T* to, float4 v) {
   *reinterpret_cast<uint2*>(to) = make_uint2(pack2<T>(v.x, v.y), pack2<T>(v.z, v.w));
 }
 
+// Eight products -> scores in log2 units.  Few of them and memory to wait for: the tanh in its general form.
+template <bool CAP>
+__device__ __forceinline__ void span_scale8(uint32_t* x, const SpanScores& c) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float s = __uint_as_float(x[e]);
+    x[e] = __float_as_uint(CAP ? c.out2 - __fdividef(2.f * c.out2, 1.f + fast_exp2(s * (2.f * kLog2e * c.in))) : s * c.scale2);
+  }
+}
+
 // CLUSTER: the parts of a row are the CTAs of a cluster
 template <typename T, int HD, bool CAP, bool BIAS, bool CLUSTER>
 __global__ void __launch_bounds__(kSdWarps * 32, 2) span_decode_kernel(const SpanDecodeParams p) {
@@ -181,7 +191,7 @@ __global__ void __launch_bounds__(kSdWarps * 32, 2) span_decode_kernel(const Spa
       uint32_t x[8];                                  // [8-key half][row, row + 8][key, key + 1]
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[e] = __float_as_uint(s[e >> 2][e & 3]);
-      span_scale<CAP, 8>(x, p.c);
+      span_scale8<CAP>(x, p.c);
       const int key0 = begin + (i * kSdWarps + warp) * kSdKeys + quad * 2;
       if constexpr (BIAS) {
 #pragma unroll
@@ -377,9 +387,7 @@ int rb_span_decode(int dtype, int head_major, const void* q, long long q_sb, lon
   SpanDecodeParams p{};
   p.q = q; p.q_sb = q_sb; p.q_sh = q_sh; p.k = k; p.v = v; p.tables = tables; p.ctx = ctx; p.starts = starts;
   p.out = out; p.part_o = part_o; p.part_lse2 = part_lse2;
-  p.c.scale2 = scale * kLog2e;
-  p.c.in = cap > 0.f ? scale / cap : 0.f;
-  p.c.out2 = cap * kLog2e;
+  p.c = rbh::span_scores(scale, cap);
   p.c.slopes = slopes;
   p.B = B; p.H = H; p.Hkv = Hkv; p.D = D; p.page = page; p.pages = pages; p.max_blocks = max_blocks; p.splits = splits; p.head_major = head_major;
   p.head_blocks = (H / Hkv + 15) / 16;

@@ -5,16 +5,19 @@
 
 namespace rb {
 
+constexpr float kLog2e = 1.4426950408889634f;
+
 struct SpanScores {
-  float scale2;        // scale log2 e (no cap)
+  float scale2;        // scale log2 e
   float in, out2;      // scale / cap, cap log2 e (cap)
+  float near;          // products up to this size are near enough to zero for the tanh's polynomial (below zero: none is)
+  float k[4];          // its coefficients in the square of a product: tanh(in s) = s (k0 + k1 s^2 + k2 s^4 + k3 s^6)
   const float* slopes; // [H] or null
   const int2* spans;   // [B, Sq] {lo, hi} or null
   long long span_batch;// rows from one batch's spans to the next's (0: all batches share them)
   int causal;
 };
 
-constexpr float kLog2e = 1.4426950408889634f;
 
 // The span of query row `row` cut to what there is: keys [x, y), {0, 0} where the row sees none.
 __device__ __forceinline__ int2 span_of(const SpanScores& c, int b, int row, int Sq, int Sk) {
@@ -28,76 +31,128 @@ __device__ __forceinline__ int2 span_of(const SpanScores& c, int b, int row, int
   return s.x < s.y ? s : make_int2(0, 0);
 }
 
-// tanh(u) = u P(u^2) for |u| <= 0.75, P of degree 4 fitted so that the largest error of tanh is least: 1.9e-7, what rounding to fp32 costs
-// beside it.  Two values at a time on the FMA pipe, where the exponential and the reciprocal of the general form would take the
-// special-function pipe, which the softmax already fills.
-constexpr float kTanhReach = 0.75f;
+__device__ __forceinline__ uint64_t pair_at(const uint32_t* s, int i) { return f32x2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])); }
+__device__ __forceinline__ void set_pair(uint32_t* s, int i, uint64_t v) {
+  const float2 f = f32x2_get(v);
+  s[i] = __float_as_uint(f.x);
+  s[i + 1] = __float_as_uint(f.y);
+}
+__device__ __forceinline__ uint64_t both(float a) { return f32x2(a, a); }
 
-// N products -> cap tanh(in s) log2 e in place.  Whole warp: one vote decides between the two forms.
-template <int N>
-__device__ __forceinline__ void span_cap(uint32_t* s, const SpanScores& c) {
-  float mx = 0.f;
-#pragma unroll
-  for (int i = 0; i < N; ++i) mx = fmaxf(mx, fabsf(__uint_as_float(s[i])));
-  if (__all_sync(0xffffffffu, mx * fabsf(c.in) <= kTanhReach)) {
-    const uint64_t in = f32x2(c.in, c.in);
-    const float fit[5] = {0.999997228f, -0.333230765f, 0.132260914f, -0.0492804431f, 0.0123188287f};
-    uint64_t k[5];
-#pragma unroll
-    for (int j = 0; j < 5; ++j) k[j] = f32x2(fit[j] * c.out2, fit[j] * c.out2);
-#pragma unroll
-    for (int i = 0; i < N; i += 2) {
-      const uint64_t u = mul_f32x2(f32x2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), in), w = mul_f32x2(u, u);
-      uint64_t r = fma_f32x2(k[4], w, k[3]);
-      r = fma_f32x2(r, w, k[2]);
-      r = fma_f32x2(r, w, k[1]);
-      r = fma_f32x2(r, w, k[0]);
-      const float2 x = f32x2_get(mul_f32x2(u, r));
-      s[i] = __float_as_uint(x.x);
-      s[i + 1] = __float_as_uint(x.y);
+// What is added to the i-th of 32 neighbouring scores of a row (or of a key): base + step i, a bias that is linear along the tile and the number that
+// the weights are relative to.  Sixteen additions of pairs from an exact beginning: what they round is below 2^-20 of the largest bias of the 32.
+struct SpanRamp {
+  float base, step;
+};
+// The same from pairs in shared memory (ADD: numbers to add, beside the ramp).
+template <bool RAMP, bool ADD>
+struct SpanAdd {
+  uint64_t at, by;
+  const float4* add;
+  __device__ __forceinline__ SpanAdd(SpanRamp r, const float4* add_) : add(add_) {
+    at = f32x2(r.base, RAMP ? r.base + r.step : r.base);
+    by = both(2.f * r.step);
+  }
+  // of places i, i + 1: called for i = 0, 2, 4, ...
+  __device__ __forceinline__ uint64_t next(int i) {
+    uint64_t v = at;
+    if (RAMP) at = add_f32x2(at, by);
+    if (ADD) {
+      const float4 f = add[i >> 2];
+      const uint64_t w = i & 2 ? f32x2(f.z, f.w) : f32x2(f.x, f.y);
+      v = RAMP ? add_f32x2(v, w) : w;
     }
-  } else {
-    const float e = 2.f * kLog2e * c.in;       // tanh u = 1 - 2 / (1 + e^2u)
-#pragma unroll
-    for (int i = 0; i < N; ++i) s[i] = __float_as_uint(c.out2 - __fdividef(2.f * c.out2, 1.f + fast_exp2(__uint_as_float(s[i]) * e)));
+    return v;
   }
+};
+
+// The polynomial: tanh(in s) out = s r(s).  Two values at a time on the FMA pipe, where the exponential and the reciprocal of the general form would take
+// the special-function pipe, which the softmax already fills.
+struct SpanTanh {
+  uint64_t k0, k1, k2, k3;
+  __device__ __forceinline__ SpanTanh(const SpanScores& c, float out) : k0(both(c.k[0] * out)), k1(both(c.k[1] * out)), k2(both(c.k[2] * out)), k3(both(c.k[3] * out)) {}
+  __device__ __forceinline__ uint64_t r(uint64_t s) const {
+    const uint64_t w = mul_f32x2(s, s);
+    return fma_f32x2(fma_f32x2(fma_f32x2(k3, w, k2), w, k1), w, k0);
+  }
+};
+// The general form, 1 - 2 / (1 + e^2u): absolute error near 1e-7
+__device__ __forceinline__ uint64_t span_tanh_any(uint32_t a, uint32_t b, const SpanScores& c) {
+  const float e = 2.f * kLog2e * c.in;
+  return f32x2(1.f - __fdividef(2.f, 1.f + fast_exp2(__uint_as_float(a) * e)), 1.f - __fdividef(2.f, 1.f + fast_exp2(__uint_as_float(b) * e)));
 }
 
-// N scores in log2 units (not shifted by distance) from products
-template <bool CAP, int N>
-__device__ __forceinline__ void span_scale(uint32_t* s, const SpanScores& c) {
-  if constexpr (CAP) {
-    span_cap<N>(s, c);
-  } else {
-    const uint64_t k = f32x2(c.scale2, c.scale2);
+__device__ __forceinline__ float span_reach32(const uint32_t* s) {
+  float mx[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < N; i += 2) {
-      const float2 x = f32x2_get(mul_f32x2(f32x2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), k));
-      s[i] = __float_as_uint(x.x);
-      s[i + 1] = __float_as_uint(x.y);
+  for (int i = 0; i < 32; ++i) mx[i & 3] = fmaxf(mx[i & 3], fabsf(__uint_as_float(s[i])));
+  return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+}
+
+// 32 products -> scores in log2 units plus what `add` gives, in place; SLIP: minus the cap's derivative, tanh^2 - 1, beside them.  `reach`: no product
+// is larger (with a cap).  Whole warp: a vote decides between the two forms of the tanh.
+template <bool CAP, bool SLIP, class Add>
+__device__ __forceinline__ void span_score32(uint32_t* s, const SpanScores& c, Add add, uint32_t* slip, float reach) {
+  if constexpr (!CAP) {
+    const uint64_t k = both(c.scale2);
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) set_pair(s, i, fma_f32x2(pair_at(s, i), k, add.next(i)));
+  } else {
+    if (__all_sync(0xffffffffu, reach <= c.near)) {
+      const SpanTanh f(c, SLIP ? 1.f : c.out2);
+#pragma unroll
+      for (int i = 0; i < 32; i += 2) {
+        const uint64_t x = pair_at(s, i), r = f.r(x);
+        if constexpr (SLIP) {
+          const uint64_t t = mul_f32x2(x, r);
+          set_pair(slip, i, fma_f32x2(t, t, both(-1.f)));
+          set_pair(s, i, fma_f32x2(t, both(c.out2), add.next(i)));
+        } else {
+          set_pair(s, i, fma_f32x2(x, r, add.next(i)));
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; i += 2) {
+        const uint64_t t = span_tanh_any(s[i], s[i + 1], c);
+        if constexpr (SLIP) set_pair(slip, i, fma_f32x2(t, t, both(-1.f)));
+        set_pair(s, i, fma_f32x2(t, both(c.out2), add.next(i)));
+      }
     }
   }
 }
 
-// x_i -= slope2 |first + i|: distances that grow by one along the tile (STEP 1) or fall by one (STEP -1).  Whole numbers up to 2^24 are exact in
-// fp32, so the only rounding is the sum's.  `side`: 1 all distances >= 0, -1 all <= 0, 0 both (warp-uniform).
-template <int STEP, int N>
-__device__ __forceinline__ void span_bias(uint32_t* s, float slope2, float first, int side) {
-  if (side != 0) {
-    const float k = side > 0 ? -slope2 : slope2;
+// s_i -= slope2 |first + step i|, for tiles with keys on both sides of their rows' places
+template <int STEP>
+__device__ __forceinline__ void span_both_sides32(uint32_t* s, float slope2, float first) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) s[i] = __float_as_uint(fmaf(k, first + (float)(STEP * i), __uint_as_float(s[i])));
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) s[i] = __float_as_uint(fmaf(-slope2, fabsf(first + (float)(STEP * i)), __uint_as_float(s[i])));
-  }
+  for (int i = 0; i < 32; ++i) s[i] = __float_as_uint(fmaf(-slope2, fabsf(first + (float)(STEP * i)), __uint_as_float(s[i])));
 }
 
+// places of 32 that `seen` does not name get `other`
+__device__ __forceinline__ void span_mask32(uint32_t* s, uint32_t seen, uint32_t other) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i)
+    if (!(seen >> i & 1)) s[i] = other;
+}
 // bit i set: place i of 32 lies in [lo, hi)
 __device__ __forceinline__ uint32_t span_bits(int lo, int hi) {
   const int a = min(max(lo, 0), 32), b = min(max(hi, 0), 32);
   const uint32_t below_b = b >= 32 ? 0xffffffffu : (1u << b) - 1, below_a = a >= 32 ? 0xffffffffu : (1u << a) - 1;
   return below_b & ~below_a;
+}
+
+// Order of a launch's CTAs: heads in groups whose keys stay in the L2 cache together, in a group the tiles from the last to the first (FROM_END; causal: the
+// longest first, so that the short ones fill the gaps at the end) or the other way, in a tile the group's heads.
+struct SpanOrder {
+  int tiles, units, group;
+};
+template <bool FROM_END>
+__device__ __forceinline__ void span_place(const SpanOrder& o, int idx, int& tile, int& unit) {
+  const int per = o.group * o.tiles, g = idx / per, in = idx - g * per, n = min(o.group, o.units - g * o.group);
+  const int t = in / n;
+  tile = FROM_END ? o.tiles - 1 - t : t;
+  unit = g * o.group + in - t * n;
 }
 
 // Range of keys that rows of a tile reach, over the `live` lanes of a warp: {least lo, largest hi, largest lo, least hi}; a row without keys keeps
@@ -118,6 +173,34 @@ __device__ __forceinline__ int4 span_range_join(int4 a, int4 b) {
 }  // namespace rb
 
 namespace rbh {
+
+// What a call's scale and cap are to the kernels.  tanh(u) = u P(u^2) for |u| <= 0.625, P of degree 3 fitted so that the largest relative error is least:
+// 3.1e-6, a hundredth of a 16-bit weight's rounding at scores of 30.  Of caps far above the scale the highest coefficients in the products are below
+// fp32's range: they are left out, and the polynomial holds as far as they make no more difference than that.  (The general form, whose error is
+// absolute, is no choice there: 1e-7 of a cap of 1e6 is 0.1.)  Of caps far below the scale they are above it, and the general form serves.
+inline rb::SpanScores span_scores(float scale, float cap) {
+  rb::SpanScores c{};
+  c.scale2 = scale * rb::kLog2e;
+  if (!(cap > 0.f)) return c;
+  c.in = scale / cap;
+  c.out2 = cap * rb::kLog2e;
+  const float a = c.in < 0.f ? -c.in : c.in, w = c.in * c.in;
+  const int terms = a > 0x1p-17f ? 4 : a > 0x1p-24f ? 3 : a > 0x1p-41f ? 2 : 1;
+  c.near = (terms == 4 ? 0.625f : terms == 3 ? 0.2f : terms == 2 ? 0.07f : 0.003f) / a;
+  if (!(c.near < 1e18f)) c.near = 1e18f;
+  if (a > 0x1p17f) c.near = -1.f;
+  c.k[0] = 0.999997256f * c.in;
+  c.k[1] = terms > 1 ? -0.333099914f * c.in * w : 0.f;
+  c.k[2] = terms > 2 ? 0.130206247f * c.in * w * w : 0.f;
+  c.k[3] = terms > 3 ? -0.040117459f * c.in * w * w * w : 0.f;
+  return c;
+}
+
+// Heads whose streamed rows (`bytes` each) take a quarter of the L2 cache
+inline int span_group(long long units, long long bytes) {
+  const long long fit = (32ll << 20) / (bytes > 0 ? bytes : 1);
+  return (int)(fit < 1 ? 1 : fit < units ? fit : units);
+}
 
 // Tensor map of heads [B, S, heads, D] with strides {batch, row, head} in elements, read in boxes of `rows` rows of 64 numbers of a head; what lies
 // beyond D reads as zero.

@@ -10,10 +10,9 @@ summed in a fixed order: the same inputs give the same gradients.
 """
 from __future__ import annotations
 
-import ctypes
 import math
 from contextlib import nullcontext
-from ctypes import c_float, c_int, c_longlong, c_void_p
+from ctypes import addressof, c_float, c_int, c_longlong, c_void_p
 from typing import Optional
 
 import torch
@@ -103,25 +102,32 @@ def kernels_take(q: torch.Tensor) -> bool:
     return q.dtype in HALVES and q.shape[-1] % 8 == 0 and 0 < q.shape[-1] <= 128
 
 
+_HERE = nullcontext()
+
+
 def _on(device):
     """Makes ``device`` the current one: launches go to its current stream."""
-    return nullcontext() if device.index in (None, torch.cuda.current_device()) else torch.cuda.device(device)
+    return _HERE if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
+
+
+_Strides = LL * 3
+
+
+def _view(t: torch.Tensor) -> torch.Tensor:
+    """The view itself if the kernels read it in place (rows of neighbouring numbers, 16-byte aligned, no dimension that repeats), else a copy."""
+    s = t.stride()
+    if s[3] == 1 and t.data_ptr() % 16 == 0 and all(n == 1 or (d > 0 and d % 8 == 0 and d < 2 ** 39) for n, d in zip(t.shape, s[:3])):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def _strides(t: torch.Tensor):
     """{batch, row, head} strides of a view as the launchers take them.  A dimension of one element has any stride; the tensor maps want a multiple
     of 16 bytes."""
-    return (LL * 3)(*(t.stride(i) if t.shape[i] > 1 else t.shape[3] for i in range(3)))
-
-
-def _view_ok(t: torch.Tensor) -> bool:
-    """Whether the kernels read this view in place: rows of neighbouring numbers, 16-byte aligned, no dimension that repeats."""
-    return (t.stride(3) == 1 or t.shape[3] == 1) and t.data_ptr() % 16 == 0 and all(
-        t.shape[i] == 1 or (t.stride(i) > 0 and t.stride(i) % 8 == 0 and t.stride(i) < 2 ** 39) for i in range(3))
-
-
-def _view(t: torch.Tensor) -> torch.Tensor:
-    return t if _view_ok(t) else t.clone(memory_format=torch.contiguous_format)
+    s, n = t.stride(), t.shape
+    if n[0] == 1 or n[1] == 1 or n[2] == 1:
+        s = [d if m > 1 else n[3] for m, d in zip(n, s)]
+    return _Strides(s[0], s[1], s[2])
 
 
 def _spans_arg(spans, rows: int):
@@ -132,20 +138,25 @@ def _spans_arg(spans, rows: int):
 
 
 # ---------------------------------------------------------------- kernels
-def span_forward(q, k, v, spans, causal: bool, scale: float, cap: float, slopes, out=None):
-    """Heads ``[B, Sq, H, D]`` and the rows' log-sum-exp in units of log 2 ``[B, H, Sq]``.  ``out``: contiguous tensor to write into."""
+def span_forward(q, k, v, spans, causal: bool, scale: float, cap: float, slopes, out=None, lse: bool = True):
+    """Heads ``[B, Sq, H, D]`` and, with ``lse``, the rows' log-sum-exp in units of log 2 ``[B, H, Sq]``.  q, k, v: views that ``_view`` returns.
+    ``out``: contiguous tensor to write into."""
     B, Sq, H, D = q.shape
     Sk, Hkv = k.shape[1], k.shape[2]
-    o = out if out is not None else torch.empty((B, Sq, H, D), dtype=q.dtype, device=q.device)
-    if not o.is_contiguous() or o.shape != q.shape or o.dtype != q.dtype or o.device != q.device or o.data_ptr() % 16:
-        raise ValueError(f"span attention writes contiguous heads {tuple(q.shape)} of {q.dtype}, not {o.dtype} {tuple(o.shape)}")
-    lse2 = torch.empty((B, H, Sq), dtype=torch.float32, device=q.device)
+    if out is None:
+        o = q.new_empty((B, Sq, H, D))
+    elif not out.is_contiguous() or out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or out.data_ptr() % 16:
+        raise ValueError(f"span attention writes contiguous heads {tuple(q.shape)} of {q.dtype}, not {out.dtype} {tuple(out.shape)}")
+    else:
+        o = out
+    lse2 = torch.empty((B, H, Sq), dtype=torch.float32, device=q.device) if lse else None
     if o.numel() == 0:
         return o, lse2
     if Sk == 0:
-        return o.zero_(), lse2.fill_(float("-inf"))
+        return o.zero_(), lse2.fill_(float("-inf")) if lse else None
     spans, batch = _spans_arg(spans, Sq)
-    slopes = None if slopes is None else slopes.contiguous()
+    if slopes is not None:
+        slopes = slopes.contiguous()
     with _on(q.device):
         L = native.lib()
         splits = L.rb_span_fwd_splits(B, H, Sq, Sk)
@@ -153,9 +164,9 @@ def span_forward(q, k, v, spans, causal: bool, scale: float, cap: float, slopes,
         if splits > 1:
             part_o = torch.empty((splits, B, Sq, H, D), dtype=torch.float32, device=q.device)
             part_lse2 = torch.empty((splits, B, H, Sq), dtype=torch.float32, device=q.device)
-        st = [_strides(t) for t in (q, k, v)]
-        check(L.rb_span_fwd(native.dtype_code(q.dtype), ptr(q), ptr(k), ptr(v), *map(ctypes.addressof, st), ptr(spans), batch, ptr(slopes), ptr(o),
-                            ptr(lse2), ptr(part_o), ptr(part_lse2), B, H, Hkv, Sq, Sk, D, splits, int(causal), float(scale), float(cap),
+        st = _strides(q), _strides(k), _strides(v)
+        check(L.rb_span_fwd(native.dtype_code(q.dtype), ptr(q), ptr(k), ptr(v), addressof(st[0]), addressof(st[1]), addressof(st[2]), ptr(spans), batch,
+                            ptr(slopes), ptr(o), ptr(lse2), ptr(part_o), ptr(part_lse2), B, H, Hkv, Sq, Sk, D, splits, int(causal), scale, cap,
                             stream_ptr()), "rb_span_fwd")
         count_launch(2 if splits > 1 else 1)
     return o, lse2
@@ -165,22 +176,21 @@ def span_backward(q, k, v, spans, causal: bool, scale: float, cap: float, slopes
     """dq, dk, dv.  ``out``: views of 16-byte aligned rows to write them into (dk and dv of the same strides)."""
     B, Sq, H, D = q.shape
     Sk, Hkv = k.shape[1], k.shape[2]
-    dq, dk, dv = out if out is not None else (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+    dq, dk, dv = out if out is not None else (q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape))
     if q.numel() == 0 or k.numel() == 0:
         return dq.zero_(), dk.zero_(), dv.zero_()
     dout = _view(dout)
     spans, batch = _spans_arg(spans, Sq)
-    slopes = None if slopes is None else slopes.contiguous()
+    if slopes is not None:
+        slopes = slopes.contiguous()
     with _on(q.device):
-        L = native.lib()
         rows = B * ((Sq + 63) // 64) * 64
         scratch = torch.empty(rows * (8 * H + 8) + rows // 64 * 16, dtype=torch.uint8, device=q.device)
-        st = [_strides(t) for t in (q, k, v)]
-        rest = [_strides(t) for t in (dout, dq, dk)]
-        at = [ctypes.addressof(s) for s in rest]
-        check(L.rb_span_bwd(native.dtype_code(q.dtype), ptr(q), ptr(k), ptr(v), *map(ctypes.addressof, st), ptr(spans), batch, ptr(slopes), ptr(o),
-                            ptr(lse2), ptr(dout), at[0], ptr(scratch), ptr(dq), ptr(dk), ptr(dv), at[1], at[2], B, H, Hkv, Sq, Sk, D, int(causal),
-                            float(scale), float(cap), stream_ptr()), "rb_span_bwd")
+        st = _strides(q), _strides(k), _strides(v), _strides(dout), _strides(dq), _strides(dk)
+        at = [addressof(s) for s in st]
+        check(native.lib().rb_span_bwd(native.dtype_code(q.dtype), ptr(q), ptr(k), ptr(v), at[0], at[1], at[2], ptr(spans), batch, ptr(slopes), ptr(o),
+                                       ptr(lse2), ptr(dout), at[3], ptr(scratch), ptr(dq), ptr(dk), ptr(dv), at[4], at[5], B, H, Hkv, Sq, Sk, D,
+                                       int(causal), scale, cap, stream_ptr()), "rb_span_bwd")
         count_launch(2)
     return dq, dk, dv
 
@@ -251,7 +261,9 @@ def span_attention(q, k, v, spans=None, causal: bool = True, scale: Optional[flo
         return span_reference(q, k, v, spans, causal, scale, cap, slopes)
     if not kernels_take(q):
         raise TypeError(f"span attention on a GPU takes bfloat16 or float16 heads of a multiple of 8 numbers up to 128, not {q.dtype} of {q.shape[-1]}")
-    return _SpanAttnFn.apply(q, k, v, spans, bool(causal), scale, cap, slopes)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return _SpanAttnFn.apply(q, k, v, spans, bool(causal), scale, cap, slopes)
+    return span_forward(_view(q), _view(k), _view(v), spans, bool(causal), scale, cap, slopes, lse=False)[0]
 
 
 def span_decode(q, k_cache, v_cache, block_tables, ctx_lens, max_ctx: int, scale: Optional[float] = None, cap: float = 0.0, slopes=None, starts=None,
@@ -283,7 +295,7 @@ def span_decode(q, k_cache, v_cache, block_tables, ctx_lens, max_ctx: int, scale
     cap = float(cap)
     _scores_ok(H, q.device, scale, cap, slopes)
     if out is None:
-        out = torch.empty((B, H, D), dtype=q.dtype, device=q.device)
+        out = q.new_empty((B, H, D))
     elif not out.is_contiguous() or out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or out.data_ptr() % 8:
         raise ValueError(f"decoding writes contiguous heads {tuple(q.shape)} of {q.dtype}, not {out.dtype} {tuple(out.shape)}")
     if not q.is_cuda:
@@ -294,11 +306,15 @@ def span_decode(q, k_cache, v_cache, block_tables, ctx_lens, max_ctx: int, scale
         raise ValueError("the caches' pages are contiguous and 16-byte aligned")
     if out.numel() == 0:
         return out
-    if q.stride(2) != 1 or q.stride(1) % 2 or q.stride(0) % 2 or q.data_ptr() % 4:
+    sb, sh, sd = q.stride()
+    if sd != 1 or sb % 2 or sh % 2 or q.data_ptr() % 4:
         q = q.clone(memory_format=torch.contiguous_format)
+        sb, sh, sd = q.stride()
     block_tables, ctx_lens = block_tables.contiguous(), ctx_lens.contiguous()
-    starts = None if starts is None else starts.contiguous()
-    slopes = None if slopes is None else slopes.contiguous()
+    if starts is not None:
+        starts = starts.contiguous()
+    if slopes is not None:
+        slopes = slopes.contiguous()
     with _on(q.device):
         L = native.lib()
         splits = L.rb_span_decode_splits(B, H, Hkv, min(int(max_ctx), block_tables.shape[1] * page, 0x7fffffff))
@@ -306,7 +322,7 @@ def span_decode(q, k_cache, v_cache, block_tables, ctx_lens, max_ctx: int, scale
         if splits > CLUSTER:
             part_o = torch.empty((splits, B, H, D), dtype=torch.float32, device=q.device)
             part_lse2 = torch.empty((splits, B, H), dtype=torch.float32, device=q.device)
-        check(L.rb_span_decode(native.dtype_code(q.dtype), int(head_major), ptr(q), q.stride(0), q.stride(1), ptr(k_cache), ptr(v_cache),
+        check(L.rb_span_decode(native.dtype_code(q.dtype), int(head_major), ptr(q), sb, sh, ptr(k_cache), ptr(v_cache),
                                ptr(block_tables), ptr(ctx_lens), ptr(starts), ptr(slopes), ptr(out), ptr(part_o), ptr(part_lse2), B, H, Hkv, D, page,
                                pages, block_tables.shape[1], splits, scale, cap, stream_ptr()), "rb_span_decode")
         count_launch(2 if splits > CLUSTER else 1)
