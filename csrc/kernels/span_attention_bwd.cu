@@ -12,6 +12,8 @@
 // of fp16 heads away from its subnormal numbers.
 #include "span_scores.cuh"
 
+#include <type_traits>
+
 namespace rb {
 
 struct SpanBwdParams {
@@ -19,16 +21,12 @@ struct SpanBwdParams {
   SpanOrder order;                  // of the launch: tiles of rows and heads, or tiles of keys and key heads
   SpanScores c;
   float grad_scale;                 // scale, negated with a cap (span_score32 gives its derivative negated)
-  const void *q, *o, *dout;         // o [B, Sq, H, D] contiguous
-  long long q_st[3], do_st[3];
   const float* lse2;                // [B, H, Sq]
   // per row, rows padded to a multiple of 64 (zeros there)
   float *row_lse2, *row_delta;      // [B, H, sq_pad], both negated
   int *row_lo, *row_hi;             // [B, sq_pad]
-  int4* range;                      // [B, sq_pad / 64] {least lo, largest hi, largest lo, least hi}
+  int4* range;                      // [B, sq_pad / 32] {least lo, largest hi, largest lo, least hi} of 32 rows
   int sq_pad;
-  void *dq, *dk, *dv;
-  long long dq_st[3], dkv_st[3];
   int* status;
 };
 
@@ -44,20 +42,24 @@ __device__ __forceinline__ void span_pack32(const uint32_t* f, uint32_t* w) {
 template <int HD>
 struct SpanDqCfg {
   static constexpr int SUB = HD / 64, SUB_BYTES = 64 * 128, TILE = SUB * SUB_BYTES;
-  static constexpr int STAGES = HD == 128 ? 6 : 8;
+  static constexpr int STAGES = HD == 128 ? 6 : 8, ROW_SUB = 128 * 128;      // 128 rows of Q, dO or O take as much as a stage: at first the last three hold them
   static constexpr int SMEM_BYTES = STAGES * 2 * TILE + 1024 + 256;
+  static_assert(SUB * ROW_SUB == 2 * TILE, "rows in the place of a stage");
   static constexpr int Q_COL = 0, DO_COL = 64, DQ_COL = 128, S_COL = 256, DP_COL = 384;     // S, dP of buffer w: + 64 w
 };
 
 template <typename T, int HD, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(320, 1)
-    span_dq_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const SpanBwdParams p) {
+    span_dq_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tdo, const __grid_constant__ CUtensorMap to,
+                   const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap tdq,
+                   const SpanBwdParams p) {
   using C = SpanDqCfg<HD>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::STAGES * 2 * C::TILE);       // [STAGES] {K, V}
-  uint64_t *full = bars, *empty = full + C::STAGES, *sdp_full = empty + C::STAGES, *ds_ready = sdp_full + 2, *dq_done = ds_ready + 2;
-  uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(dq_done + 1);
+  uint64_t *full = bars, *empty = full + C::STAGES, *sdp_full = empty + C::STAGES, *ds_ready = sdp_full + 2, *dq_done = ds_ready + 2,
+           *rows_full = dq_done + 1, *rows_read = rows_full + 1;
+  uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(rows_read + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_ptr + 1);
   __shared__ int4 s_range[4];
   __shared__ float s_delta[128];
@@ -82,8 +84,20 @@ __global__ void __launch_bounds__(320, 1)
       mbar_init(smem_u32(&ds_ready[w]), 128);
     }
     mbar_init(smem_u32(dq_done), 1);
+    mbar_init(smem_u32(rows_full), 1);
+    mbar_init(smem_u32(rows_read), 256);
     *abort_flag = 0;
     fence_barrier_init();
+    fence_proxy_async();
+    // this thread's own barriers: the copies need no one else
+    mbar_arrive_expect_tx(smem_u32(rows_full), 3 * 2 * C::TILE);
+    uint8_t* rows = smem + (C::STAGES - 3) * 2 * C::TILE;
+#pragma unroll
+    for (int s = 0; s < C::SUB; ++s) {
+      tma_load_4d(smem_u32(rows + s * C::ROW_SUB), &tq, smem_u32(rows_full), s * 64, q0, h, b);
+      tma_load_4d(smem_u32(rows + 2 * C::TILE + s * C::ROW_SUB), &tdo, smem_u32(rows_full), s * 64, q0, h, b);
+      tma_load_4d(smem_u32(rows + 4 * C::TILE + s * C::ROW_SUB), &to, smem_u32(rows_full), s * 64, q0, h, b);
+    }
   }
   int2 span = make_int2(0, 0);
   if (warp < 8) {
@@ -98,39 +112,41 @@ __global__ void __launch_bounds__(320, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_ptr;
-  const int4 half0 = span_range_join(s_range[0], s_range[1]), half1 = span_range_join(s_range[2], s_range[3]);
-  const int4 all = span_range_join(half0, half1);
+  const int4 all = span_range_join(span_range_join(s_range[0], s_range[1]), span_range_join(s_range[2], s_range[3]));
   const int j0 = all.x < all.y ? all.x / 64 : 0, n = all.x < all.y ? (all.y + 63) / 64 - j0 : 0;
 
   const uint32_t lane_addr = tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16);
   float lse2 = 0.f;
+  bool ok = true;
   if (warp < 8) {
-    // Q (first warpgroup) and dO (second) into tensor memory; delta on the way
-    const T* from = wg == 0 ? reinterpret_cast<const T*>(p.q) + b * p.q_st[0] + row * p.q_st[1] + h * p.q_st[2]
-                            : reinterpret_cast<const T*>(p.dout) + b * p.do_st[0] + row * p.do_st[1] + h * p.do_st[2];
-    const T* o = reinterpret_cast<const T*>(p.o) + ((static_cast<long long>(b) * p.Sq + row) * p.H + h) * p.D;
+    // Q (first warpgroup) and dO (second) into tensor memory; delta on the way.  By way of shared memory: a thread's own row of loads, 16 bytes of a line
+    // each, took 10000 cycles.
+    ok = mbar_wait(smem_u32(rows_full), 0, abort_flag, p.status, RB_ERR_TIMEOUT_FULL);
+    ok = __all_sync(0xffffffffu, ok);
+    const uint8_t* from = smem + (C::STAGES - 3 + wg) * 2 * C::TILE + t * 128;
+    const uint8_t* o = smem + (C::STAGES - 1) * 2 * C::TILE + t * 128;
     float delta = 0.f;
 #pragma unroll
     for (int c = 0; c < HD / 32; ++c) {
       uint32_t w[16];
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        uint4 v = make_uint4(0, 0, 0, 0), y = v;
-        const int d = c * 32 + g * 8;
-        if (live && d < p.D) {
-          v = *reinterpret_cast<const uint4*>(from + d);
-          if (wg == 1) y = *reinterpret_cast<const uint4*>(o + d);
-        }
+        const int d = c * 32 + g * 8, at = (d >> 6) * C::ROW_SUB + ((((d >> 3) & 7) ^ (t & 7)) << 4);
+        const uint4 v = *reinterpret_cast<const uint4*>(from + at);
         w[g * 4] = v.x; w[g * 4 + 1] = v.y; w[g * 4 + 2] = v.z; w[g * 4 + 3] = v.w;
-        const uint32_t z[4] = {y.x, y.y, y.z, y.w};
+        if (wg == 1) {
+          const uint4 y = *reinterpret_cast<const uint4*>(o + at);
+          const uint32_t z[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 e = unpack2<T>(w[g * 4 + i]), f = unpack2<T>(z[i]);
-          delta = fmaf(e.x, f.x, fmaf(e.y, f.y, delta));
+          for (int i = 0; i < 4; ++i) {
+            const float2 e = unpack2<T>(w[g * 4 + i]), f = unpack2<T>(z[i]);
+            delta = fmaf(e.x, f.x, fmaf(e.y, f.y, delta));
+          }
         }
       }
       tmem_st_32x32b_x16(lane_addr + (wg == 0 ? C::Q_COL : C::DO_COL) + c * 16, w);
     }
+    mbar_arrive(smem_u32(rows_read));
     if (live && span.x < span.y) lse2 = p.lse2[(static_cast<long long>(b) * p.H + h) * p.Sq + row];
     if (row < p.sq_pad) {
       const long long at = (static_cast<long long>(b) * p.H + h) * p.sq_pad + row;
@@ -139,10 +155,10 @@ __global__ void __launch_bounds__(320, 1)
       if (h == 0 && wg == 0) {
         p.row_lo[static_cast<long long>(b) * p.sq_pad + row] = span.x;
         p.row_hi[static_cast<long long>(b) * p.sq_pad + row] = span.y;
-        if ((t & 63) == 0) {
-          int4 r = t == 0 ? half0 : half1;
-          if (row + 64 > p.Sq) r.w = 0;           // rows behind the last one see nothing: such a tile is masked
-          p.range[(static_cast<long long>(b) * p.sq_pad + row) / 64] = r;
+        if (lane == 0) {
+          int4 r = s_range[warp];
+          if (row + 32 > p.Sq) r.w = 0;           // rows behind the last one see nothing: their scores are masked
+          p.range[(static_cast<long long>(b) * p.sq_pad + row) / 32] = r;
         }
       }
     }
@@ -156,11 +172,11 @@ __global__ void __launch_bounds__(320, 1)
   if (warp == 8) {
     // ------------------------------ TMA producer ------------------------------
     if (lane == 0) {
-      bool ok = true;
       int st = 0;
       uint32_t ph = 0;
       for (int i = 0; i < n; ++i) {
-        ok = mbar_wait(smem_u32(&empty[st]), ph ^ 1, abort_flag, p.status, RB_ERR_TIMEOUT_EMPTY);
+        ok = i == C::STAGES - 3 ? mbar_wait(smem_u32(rows_read), 0, abort_flag, p.status, RB_ERR_TIMEOUT_EMPTY)
+                                : mbar_wait(smem_u32(&empty[st]), ph ^ 1, abort_flag, p.status, RB_ERR_TIMEOUT_EMPTY);
         if (!ok) break;
         const uint32_t bar = smem_u32(&full[st]), dst = smem_u32(smem + st * 2 * C::TILE);
         mbar_arrive_expect_tx(bar, 2 * C::TILE);
@@ -178,7 +194,6 @@ __global__ void __launch_bounds__(320, 1)
     // ------------------------------ MMA issuer --------------------------------
     constexpr uint32_t idesc_s = make_idesc(UmmaFormat<T>::value, 0, 0, 128, 64);
     constexpr uint32_t idesc_q = make_idesc(UmmaFormat<T>::value, 0, 1, 128, HD);
-    bool ok = true;
     int st_in = 0, st_out = 0;
     uint32_t ph_in = 0;
     auto issue = [&](int i) {            // S and dP of tile i, the next stage
@@ -211,8 +226,7 @@ __global__ void __launch_bounds__(320, 1)
     // ------------------------------ softmax warpgroups ------------------------
     const float slope2 = BIAS ? p.c.slopes[h] * kLog2e : 0.f, delta = s_delta[t];
     const uint32_t s_addr = lane_addr + C::S_COL + wg * 64, dp_addr = lane_addr + C::DP_COL + wg * 64;
-    bool ok = true;
-    for (int i = wg; i < n; i += 2) {
+    for (int i = wg; i < n && ok; i += 2) {
       ok = mbar_wait(smem_u32(&sdp_full[wg]), (i >> 1) & 1, abort_flag, p.status, RB_ERR_TIMEOUT_TMEM_FULL);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
@@ -223,14 +237,14 @@ __global__ void __launch_bounds__(320, 1)
       const float slope = side > 0 ? slope2 : -slope2;
       const uint64_t minus = both(-delta);
       uint32_t ds[2][16];
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
+      // dS of chunk c of 32 keys; PART: some of them are unseen
+      auto chunk = [&](int c, auto part, uint32_t seen) {
+        constexpr bool PART = decltype(part)::value;
         uint32_t s[32], dp[32], slip[32];
         tmem_ld_32x32b_x32(s_addr + c * 32, s);
         tmem_ld_32x32b_x32(dp_addr + c * 32, dp);
         tmem_ld_wait();
-        const uint32_t seen = masked ? span_bits(span.x - kv0 - c * 32, span.y - kv0 - c * 32) : 0xffffffffu;
-        if (masked) span_mask32(s, seen, 0);         // what unseen keys hold decides nothing
+        if (PART) span_mask32(s, seen, 0);           // what unseen keys hold decides nothing
         const float first = (float)(row + off - kv0 - c * 32), reach = CAP ? span_reach32(s) : 0.f;
         if (BIAS && side != 0) {
           span_score32<CAP, true>(s, p.c, SpanAdd<true, false>({fmaf(-slope, first, -lse2), slope}, nullptr), slip, reach);
@@ -244,8 +258,24 @@ __global__ void __launch_bounds__(320, 1)
           if (CAP) w = mul_f32x2(w, pair_at(slip, k));
           set_pair(s, k, mul_f32x2(w, add_f32x2(pair_at(dp, k), minus)));
         }
-        if (masked) span_mask32(s, seen, 0);
+        if (PART) span_mask32(s, seen, 0);
         span_pack32<T>(s, ds[c]);
+      };
+      if (!masked) {
+        chunk(0, std::false_type{}, 0xffffffffu);
+        chunk(1, std::false_type{}, 0xffffffffu);
+      } else {
+        // some chunks of a masked tile have nothing to see
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const uint32_t seen = span_bits(span.x - kv0 - c * 32, span.y - kv0 - c * 32);
+          if (__all_sync(0xffffffffu, seen == 0)) {
+#pragma unroll
+            for (int k = 0; k < 16; ++k) ds[c][k] = 0;
+          } else {
+            chunk(c, std::true_type{}, seen);
+          }
+        }
       }
       tmem_st_32x32b_x16(s_addr, ds[0]);
       tmem_st_32x32b_x16(s_addr + 16, ds[1]);
@@ -259,12 +289,11 @@ __global__ void __launch_bounds__(320, 1)
       tc_fence_after();
     }
     if (ok) {
-      // warpgroup w stores columns [w HD / 2, (w + 1) HD / 2)
-      T* out = reinterpret_cast<T*>(p.dq) + b * p.dq_st[0] + row * p.dq_st[1] + h * p.dq_st[2];
+      // warpgroup w takes columns [w HD / 2, (w + 1) HD / 2): through shared memory (all copies have landed and been used), from there in whole rows
+      uint8_t* stage = smem + t * 128;
 #pragma unroll 1
       for (int c = 0; c < HD / 64; ++c) {
         const int d0 = wg * (HD / 2) + c * 32;
-        if (d0 >= p.D) break;
         uint32_t r[32];
         if (n > 0) {
           tmem_ld_32x32b_x32(lane_addr + C::DQ_COL + d0, r);
@@ -273,16 +302,24 @@ __global__ void __launch_bounds__(320, 1)
 #pragma unroll
           for (int k = 0; k < 32; ++k) r[k] = 0;
         }
-        if (!live) continue;
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          if (d0 + g * 8 >= p.D) break;
+          const int d = d0 + g * 8;
           uint32_t w[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k) w[k] = pack2<T>(__uint_as_float(r[g * 8 + 2 * k]) * p.grad_scale, __uint_as_float(r[g * 8 + 2 * k + 1]) * p.grad_scale);
-          *reinterpret_cast<uint4*>(out + d0 + g * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+          *reinterpret_cast<uint4*>(stage + (d >> 6) * C::ROW_SUB + ((((d >> 3) & 7) ^ (t & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
         }
       }
+    }
+    fence_proxy_async_smem();
+    asm volatile("bar.sync 1, 256;" ::: "memory");          // the softmax warps, also where a wait ran out
+    if (threadIdx.x == 0 && ok) {
+#pragma unroll
+      for (int s = 0; s < C::SUB; ++s)
+        if (s * 64 < p.D) tma_store_4d(&tdq, smem_u32(smem + s * C::ROW_SUB), s * 64, q0, h, b);
+      tma_store_commit();
+      tma_store_wait_read<0>();
     }
   }
 
@@ -311,7 +348,8 @@ struct SpanDkvCfg {
 template <typename T, int HD, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(320, 1)
     span_dkv_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
-                    const __grid_constant__ CUtensorMap tdo, const SpanBwdParams p) {
+                    const __grid_constant__ CUtensorMap tdo, const __grid_constant__ CUtensorMap tdk, const __grid_constant__ CUtensorMap tdv,
+                    const SpanBwdParams p) {
   using C = SpanDkvCfg<HD>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -330,7 +368,7 @@ __global__ void __launch_bounds__(320, 1)
   span_place<false>(p.order, blockIdx.x, kv_tile, unit);      // causal: the keys that most rows see first
   const int kv0 = kv_tile * 128, hkv = unit % p.Hkv, b = unit / p.Hkv, group = p.H / p.Hkv;
   const int off = p.Sk - p.Sq, q_tiles = p.sq_pad / 64;
-  const int4* range = p.range + static_cast<long long>(b) * q_tiles;
+  const int4* range = p.range + static_cast<long long>(b) * q_tiles * 2;
 
   if (threadIdx.x == 0) {
     prefetch_tensormap(&tq);
@@ -362,7 +400,7 @@ __global__ void __launch_bounds__(320, 1)
   const uint32_t tmem_base = *tmem_ptr;
   // query tiles from the first to the last that reaches these keys (what lies between and does not is masked)
   for (int i = threadIdx.x; i < q_tiles; i += 320) {
-    const int4 r = range[i];
+    const int4 r = span_range_join(range[2 * i], range[2 * i + 1]);
     if (r.x < kv0 + 128 && r.y > kv0) {
       atomicMin(&s_first, i);
       atomicMax(&s_last, i);
@@ -371,11 +409,17 @@ __global__ void __launch_bounds__(320, 1)
   __syncthreads();
   const int tile0 = s_first, per_head = s_last < 0 ? 0 : s_last + 1 - tile0;
   const int n = per_head * group;
-  auto coords = [&](int it, int& h, int& tile) {
-    const int g = it / per_head;
-    h = hkv * group + g;
-    tile = tile0 + it - g * per_head;
+  // the sweep's tiles in turn: query tiles of the first head, then of the next
+  struct Place {
+    int h, tile;
   };
+  auto next = [&](Place& c) {
+    if (++c.tile == tile0 + per_head) {
+      c.tile = tile0;
+      ++c.h;
+    }
+  };
+  const Place start = {hkv * group, tile0};
 
   if (warp == 8) {
     // ------------------------------ TMA producer ------------------------------
@@ -389,11 +433,11 @@ __global__ void __launch_bounds__(320, 1)
       bool ok = true;
       int st = 0;
       uint32_t ph = 0;
-      for (int it = 0; it < n; ++it) {
+      Place at = start;
+      for (int it = 0; it < n; ++it, next(at)) {
         ok = mbar_wait(smem_u32(&empty[st]), ph ^ 1, abort_flag, p.status, RB_ERR_TIMEOUT_EMPTY);
         if (!ok) break;
-        int h, tile;
-        coords(it, h, tile);
+        const int h = at.h, tile = at.tile;
         const uint32_t bar = smem_u32(&full[st]), dst = smem_u32(sQ + st * 2 * C::Q_TILE), rows = smem_u32(sRow + st * 1024);
         mbar_arrive_expect_tx(bar, 2 * C::Q_TILE + 1024);
         const long long bh = (static_cast<long long>(b) * p.H + h) * p.sq_pad + tile * 64, bb = static_cast<long long>(b) * p.sq_pad + tile * 64;
@@ -461,16 +505,22 @@ __global__ void __launch_bounds__(320, 1)
     const uint32_t lane_addr = tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     bool ok = true;
     int st = 0;
-    int4 here = n > 0 ? range[tile0] : make_int4(0, 0, 0, 0);
+    Place at = start;
+    int4 here = make_int4(0, 0, 0, 0);            // of the tile: asked for one tile ahead
+    float slope_here = 0.f;
+    auto ask = [&]() {
+      here = range[2 * at.tile + half];
+      if (BIAS) slope_here = __ldg(p.c.slopes + at.h);
+    };
+    if (n > 0) ask();
     for (int it = 0; it < n; ++it) {
-      int h, tile, h2, tile2 = 0;
-      coords(it, h, tile);
+      const int tile = at.tile;
       const int4 r = here;
+      const float slope2 = slope_here * kLog2e;
       if (it + 1 < n) {
-        coords(it + 1, h2, tile2);
-        here = range[tile2];
+        next(at);
+        ask();
       }
-      const float slope2 = BIAS ? __ldg(p.c.slopes + h) * kLog2e : 0.f;
       ok = mbar_wait(smem_u32(&st_full[it & 1]), (it >> 1) & 1, abort_flag, p.status, RB_ERR_TIMEOUT_TMEM_FULL);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
@@ -480,47 +530,57 @@ __global__ void __launch_bounds__(320, 1)
       if (++st == C::STAGES) st = 0;
       const float4 *lse4 = reinterpret_cast<const float4*>(rows), *delta4 = reinterpret_cast<const float4*>(rows + 256);
       const int4 *lo4 = reinterpret_cast<const int4*>(rows + 512), *hi4 = reinterpret_cast<const int4*>(rows + 768);
-      const bool masked = kv0 < r.z || kv0 + 128 > r.w;
+      // the warp's 32 keys and these 32 rows: nothing seen, or all
+      const int key0 = kv0 + (warp & 3) * 32;
+      const bool none = key0 + 32 <= r.x || key0 >= r.y, part = !none && (key0 < r.z || key0 + 32 > r.w);
       const int first = tile * 64 + off;                        // place of the tile's first row among the keys
       const int side = !BIAS ? 1 : p.c.causal || first >= kv0 + 127 ? 1 : first + 63 <= kv0 ? -1 : 0;
       const uint32_t st_addr = lane_addr + C::ST_COL + (it & 1) * 64 + half * 32;
-      uint32_t s[32], dp[32], slip[32], packed[16];
-      tmem_ld_32x32b_x32(st_addr, s);
-      tmem_ld_32x32b_x32(lane_addr + C::DP_COL + (it & 1) * 64 + half * 32, dp);
-      tmem_ld_wait();
-      uint32_t seen = 0xffffffffu;
-      if (masked) {
-        seen = 0;
+      uint32_t packed[16];
+      if (none) {
 #pragma unroll
-        for (int i4 = 0; i4 < 8; ++i4) {
-          const int4 lo = lo4[i4], hi = hi4[i4];
-          seen |= (kv >= lo.x && kv < hi.x ? 1u : 0u) << (i4 * 4) | (kv >= lo.y && kv < hi.y ? 2u : 0u) << (i4 * 4) |
-                  (kv >= lo.z && kv < hi.z ? 4u : 0u) << (i4 * 4) | (kv >= lo.w && kv < hi.w ? 8u : 0u) << (i4 * 4);
-        }
-        span_mask32(s, seen, 0);         // what unseen keys hold decides nothing
-      }
-      const float away = (float)(first + half * 32 - kv), slope = side > 0 ? -slope2 : slope2, reach = CAP ? span_reach32(s) : 0.f;
-      if (BIAS && side != 0) {
-        span_score32<CAP, true>(s, p.c, SpanAdd<true, true>({slope * away, slope}, lse4), slip, reach);
+        for (int k = 0; k < 16; ++k) packed[k] = 0;
+        tmem_st_32x32b_x16(st_addr, packed);
+        tmem_st_32x32b_x16(st_addr + 16, packed);
       } else {
-        span_score32<CAP, true>(s, p.c, SpanAdd<false, true>({0.f, 0.f}, lse4), slip, reach);
-        if constexpr (BIAS) span_both_sides32<1>(s, slope2, away);
-      }
+        uint32_t s[32], dp[32], slip[32];
+        tmem_ld_32x32b_x32(st_addr, s);
+        tmem_ld_32x32b_x32(lane_addr + C::DP_COL + (it & 1) * 64 + half * 32, dp);
+        tmem_ld_wait();
+        uint32_t seen = 0xffffffffu;
+        if (part) {
+          seen = 0;
 #pragma unroll
-      for (int k = 0; k < 32; ++k) s[k] = __float_as_uint(fast_exp2(__uint_as_float(s[k])));
-      if (masked) span_mask32(s, seen, 0);
-      span_pack32<T>(s, packed);
-      tmem_st_32x32b_x16(st_addr, packed);
+          for (int i4 = 0; i4 < 8; ++i4) {
+            const int4 lo = lo4[i4], hi = hi4[i4];
+            seen |= (kv >= lo.x && kv < hi.x ? 1u : 0u) << (i4 * 4) | (kv >= lo.y && kv < hi.y ? 2u : 0u) << (i4 * 4) |
+                    (kv >= lo.z && kv < hi.z ? 4u : 0u) << (i4 * 4) | (kv >= lo.w && kv < hi.w ? 8u : 0u) << (i4 * 4);
+          }
+          span_mask32(s, seen, 0);         // what unseen keys hold decides nothing
+        }
+        const float away = (float)(first + half * 32 - kv), slope = side > 0 ? -slope2 : slope2, reach = CAP ? span_reach32(s) : 0.f;
+        if (BIAS && side != 0) {
+          span_score32<CAP, true>(s, p.c, SpanAdd<true, true>({slope * away, slope}, lse4), slip, reach);
+        } else {
+          span_score32<CAP, true>(s, p.c, SpanAdd<false, true>({0.f, 0.f}, lse4), slip, reach);
+          if constexpr (BIAS) span_both_sides32<1>(s, slope2, away);
+        }
 #pragma unroll
-      for (int k = 0; k < 32; k += 2) {
-        const float4 d = delta4[k >> 2];
-        uint64_t w = pair_at(s, k);
-        if (CAP) w = mul_f32x2(w, pair_at(slip, k));
-        set_pair(s, k, mul_f32x2(w, add_f32x2(pair_at(dp, k), k & 2 ? f32x2(d.z, d.w) : f32x2(d.x, d.y))));
+        for (int k = 0; k < 32; ++k) s[k] = __float_as_uint(fast_exp2(__uint_as_float(s[k])));
+        if (part) span_mask32(s, seen, 0);
+        span_pack32<T>(s, packed);
+        tmem_st_32x32b_x16(st_addr, packed);
+#pragma unroll
+        for (int k = 0; k < 32; k += 2) {
+          const float4 d = delta4[k >> 2];
+          uint64_t w = pair_at(s, k);
+          if (CAP) w = mul_f32x2(w, pair_at(slip, k));
+          set_pair(s, k, mul_f32x2(w, add_f32x2(pair_at(dp, k), k & 2 ? f32x2(d.z, d.w) : f32x2(d.x, d.y))));
+        }
+        if (part) span_mask32(s, seen, 0);
+        span_pack32<T>(s, packed);
+        tmem_st_32x32b_x16(st_addr + 16, packed);
       }
-      if (masked) span_mask32(s, seen, 0);
-      span_pack32<T>(s, packed);
-      tmem_st_32x32b_x16(st_addr + 16, packed);
       tmem_st_wait();
       tc_fence_before();
       mbar_arrive(smem_u32(&ready[it & 1]));
@@ -531,12 +591,11 @@ __global__ void __launch_bounds__(320, 1)
       tc_fence_after();
     }
     if (ok) {
-      // warps 0-3 store dV, warps 4-7 dK
-      T* out = reinterpret_cast<T*>(half == 0 ? p.dv : p.dk) + b * p.dkv_st[0] + kv * p.dkv_st[1] + hkv * p.dkv_st[2];
+      // warps 0-3 take dV, warps 4-7 dK: through shared memory, in the place of V and K, from there in whole rows
+      uint8_t* stage = (half == 0 ? sV : sK) + t * 128;
       const float f = half == 0 ? 1.f : p.grad_scale;
 #pragma unroll 1
       for (int c = 0; c < HD / 32; ++c) {
-        if (c * 32 >= p.D) break;
         uint32_t r[32];
         if (n > 0) {
           tmem_ld_32x32b_x32(lane_addr + (half == 0 ? C::DV_COL : C::DK_COL) + c * 32, r);
@@ -545,16 +604,24 @@ __global__ void __launch_bounds__(320, 1)
 #pragma unroll
           for (int k = 0; k < 32; ++k) r[k] = 0;
         }
-        if (kv >= p.Sk) continue;
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          if (c * 32 + g * 8 >= p.D) break;
+          const int d = c * 32 + g * 8;
           uint32_t w[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k) w[k] = pack2<T>(__uint_as_float(r[g * 8 + 2 * k]) * f, __uint_as_float(r[g * 8 + 2 * k + 1]) * f);
-          *reinterpret_cast<uint4*>(out + c * 32 + g * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+          *reinterpret_cast<uint4*>(stage + (d >> 6) * C::KV_SUB + ((((d >> 3) & 7) ^ (t & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
         }
       }
+    }
+    fence_proxy_async_smem();
+    asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory");          // these four warps, also where a wait ran out
+    if (t == 0 && ok) {
+#pragma unroll
+      for (int s = 0; s < C::SUB; ++s)
+        if (s * 64 < p.D) tma_store_4d(half == 0 ? &tdv : &tdk, smem_u32((half == 0 ? sV : sK) + s * C::KV_SUB), s * 64, kv0, hkv, b);
+      tma_store_commit();
+      tma_store_wait_read<0>();
     }
   }
 
@@ -566,8 +633,13 @@ __global__ void __launch_bounds__(320, 1)
   }
 }
 
+struct SpanBwdArrays {
+  const void *q, *k, *v, *o, *dout, *dq, *dk, *dv;        // o [B, Sq, H, D] contiguous
+  const long long *qs, *ks, *vs, *dos, *dqs, *dkvs;
+};
+// Tensor maps: rows of queries, gradients and results in boxes of 64 and 128 rows, keys and values too
 struct SpanBwdMaps {
-  CUtensorMap q, k, v, dout, k64, v64;
+  CUtensorMap q64, q128, do64, do128, o128, dq128, k64, k128, v64, v128, dk128, dv128;
 };
 
 template <typename T, int HD, bool CAP, bool BIAS>
@@ -580,22 +652,36 @@ int launch_span_bwd(const SpanBwdMaps& m, SpanBwdParams p, cudaStream_t st) {
   const long long q_tiles = (p.Sq + 127) / 128, kv_tiles = (p.Sk + 127) / 128;
   if (q_tiles * p.H * p.B > 0x7fffffffll || kv_tiles * p.Hkv * p.B > 0x7fffffffll) return 20;
   p.order = {(int)q_tiles, p.H * p.B, rbh::span_group(static_cast<long long>(p.H) * p.B, 4ll * p.Sk * p.D * p.Hkv / p.H)};
-  dq<<<(unsigned)(q_tiles * p.H * p.B), 320, SpanDqCfg<HD>::SMEM_BYTES, st>>>(m.k64, m.v64, p);
+  dq<<<(unsigned)(q_tiles * p.H * p.B), 320, SpanDqCfg<HD>::SMEM_BYTES, st>>>(m.q128, m.do128, m.o128, m.k64, m.v64, m.dq128, p);
   p.order = {(int)kv_tiles, p.Hkv * p.B, rbh::span_group(static_cast<long long>(p.Hkv) * p.B, 4ll * p.Sq * p.D * (p.H / p.Hkv))};
-  dkv<<<(unsigned)(kv_tiles * p.Hkv * p.B), 320, SpanDkvCfg<HD>::SMEM_BYTES, st>>>(m.q, m.k, m.v, m.dout, p);
+  dkv<<<(unsigned)(kv_tiles * p.Hkv * p.B), 320, SpanDkvCfg<HD>::SMEM_BYTES, st>>>(m.q64, m.k128, m.v128, m.do64, m.dk128, m.dv128, p);
   e = cudaGetLastError();
   return e == cudaSuccess ? 0 : 3000 + (int)e;
 }
 
 template <typename T>
-int span_bwd(int dtype, const void* k, const void* v, const long long* ks, const long long* vs, const SpanBwdParams& p, bool cap, cudaStream_t st) {
+int span_bwd(int dtype, const SpanBwdArrays& a, const SpanBwdParams& p, bool cap, cudaStream_t st) {
   SpanBwdMaps m;
-  int rc = rbh::span_map(&m.q, dtype, p.q, p.q_st, p.B, p.Sq, p.H, p.D, 64);
-  if (!rc) rc = rbh::span_map(&m.dout, dtype, p.dout, p.do_st, p.B, p.Sq, p.H, p.D, 64);
-  if (!rc) rc = rbh::span_map(&m.k, dtype, k, ks, p.B, p.Sk, p.Hkv, p.D, 128);
-  if (!rc) rc = rbh::span_map(&m.v, dtype, v, vs, p.B, p.Sk, p.Hkv, p.D, 128);
-  if (!rc) rc = rbh::span_map(&m.k64, dtype, k, ks, p.B, p.Sk, p.Hkv, p.D, 64);
-  if (!rc) rc = rbh::span_map(&m.v64, dtype, v, vs, p.B, p.Sk, p.Hkv, p.D, 64);
+  const long long os[3] = {static_cast<long long>(p.Sq) * p.H * p.D, static_cast<long long>(p.H) * p.D, p.D};
+  int rc = 0;
+  auto rows = [&](CUtensorMap* map, const void* base, const long long* s, int box) {
+    if (!rc) rc = rbh::span_map(map, dtype, base, s, p.B, p.Sq, p.H, p.D, box);
+  };
+  auto keys = [&](CUtensorMap* map, const void* base, const long long* s, int box) {
+    if (!rc) rc = rbh::span_map(map, dtype, base, s, p.B, p.Sk, p.Hkv, p.D, box);
+  };
+  rows(&m.q64, a.q, a.qs, 64);
+  rows(&m.q128, a.q, a.qs, 128);
+  rows(&m.do64, a.dout, a.dos, 64);
+  rows(&m.do128, a.dout, a.dos, 128);
+  rows(&m.o128, a.o, os, 128);
+  rows(&m.dq128, a.dq, a.dqs, 128);
+  keys(&m.k64, a.k, a.ks, 64);
+  keys(&m.k128, a.k, a.ks, 128);
+  keys(&m.v64, a.v, a.vs, 64);
+  keys(&m.v128, a.v, a.vs, 128);
+  keys(&m.dk128, a.dk, a.dkvs, 128);
+  keys(&m.dv128, a.dv, a.dkvs, 128);
   if (rc) return 1000 + rc;
   const bool bias = p.c.slopes != nullptr;
 #define RB_SPAN(HD_)                                                                                               \
@@ -610,7 +696,7 @@ int span_bwd(int dtype, const void* k, const void* v, const long long* ks, const
 extern "C" {
 
 // Gradients of rb_span_fwd.  q, k, v, dout: 16-bit views as there; o contiguous and lse2 from the forward call with the same arguments.  dq [B, Sq, H, D]; dk and
-// dv [B, Sk, Hkv, D] of the same strides: views of 16-byte aligned rows.  scratch: 16-byte aligned, B pad (8 H + 8) + B pad / 4 bytes with pad = Sq rounded up to
+// dv [B, Sk, Hkv, D] of the same strides: views of 16-byte aligned rows.  scratch: 16-byte aligned, B pad (8 H + 8) + B pad / 2 bytes with pad = Sq rounded up to
 // a multiple of 64; nothing in it has to be set.
 int rb_span_bwd(int dtype, const void* q, const void* k, const void* v, const long long* qs, const long long* ks, const long long* vs, const int* spans,
                 long long span_batch, const float* slopes, const void* o, const float* lse2, const void* dout, const long long* dos, void* scratch, void* dq,
@@ -627,8 +713,7 @@ int rb_span_bwd(int dtype, const void* q, const void* k, const void* v, const lo
   p.c.span_batch = span_batch;
   p.c.causal = causal;
   p.grad_scale = cap > 0.f ? -scale : scale;
-  p.q = q; p.o = o; p.dout = dout; p.lse2 = lse2;
-  for (int i = 0; i < 3; ++i) { p.q_st[i] = qs[i]; p.do_st[i] = dos[i]; p.dq_st[i] = dqs[i]; p.dkv_st[i] = dkvs[i]; }
+  p.lse2 = lse2;
   p.sq_pad = (Sq + 63) / 64 * 64;
   const long long rows = static_cast<long long>(B) * p.sq_pad;
   p.row_lse2 = reinterpret_cast<float*>(scratch);
@@ -636,11 +721,11 @@ int rb_span_bwd(int dtype, const void* q, const void* k, const void* v, const lo
   p.row_lo = reinterpret_cast<int*>(p.row_delta + rows * H);
   p.row_hi = p.row_lo + rows;
   p.range = reinterpret_cast<int4*>(p.row_hi + rows);
-  p.dq = dq; p.dk = dk; p.dv = dv;
+  const SpanBwdArrays a = {q, k, v, o, dout, dq, dk, dv, qs, ks, vs, dos, dqs, dkvs};
   p.status = rbh::device_status_word();
   cudaStream_t st = (cudaStream_t)stream;
-  if (dtype == rbh::DT_BF16) return span_bwd<__nv_bfloat16>(dtype, k, v, ks, vs, p, cap > 0.f, st);
-  if (dtype == rbh::DT_F16) return span_bwd<__half>(dtype, k, v, ks, vs, p, cap > 0.f, st);
+  if (dtype == rbh::DT_BF16) return span_bwd<__nv_bfloat16>(dtype, a, p, cap > 0.f, st);
+  if (dtype == rbh::DT_F16) return span_bwd<__half>(dtype, a, p, cap > 0.f, st);
   return 20;
 }
 }

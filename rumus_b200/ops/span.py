@@ -115,19 +115,22 @@ _Strides = LL * 3
 
 def _view(t: torch.Tensor) -> torch.Tensor:
     """The view itself if the kernels read it in place (rows of neighbouring numbers, 16-byte aligned, no dimension that repeats), else a copy."""
-    s = t.stride()
-    if s[3] == 1 and t.data_ptr() % 16 == 0 and all(n == 1 or (d > 0 and d % 8 == 0 and d < 2 ** 39) for n, d in zip(t.shape, s[:3])):
-        return t
+    b, r, h, one = t.stride()
+    if one == 1 and t.data_ptr() % 16 == 0:
+        if not (b | r | h) & 7 and 0 < b < 2 ** 39 and 0 < r < 2 ** 39 and 0 < h < 2 ** 39:
+            return t
+        if all(n == 1 or (d > 0 and d % 8 == 0 and d < 2 ** 39) for n, d in zip(t.shape, (b, r, h))):
+            return t
     return t.clone(memory_format=torch.contiguous_format)
 
 
 def _strides(t: torch.Tensor):
     """{batch, row, head} strides of a view as the launchers take them.  A dimension of one element has any stride; the tensor maps want a multiple
     of 16 bytes."""
-    s, n = t.stride(), t.shape
-    if n[0] == 1 or n[1] == 1 or n[2] == 1:
-        s = [d if m > 1 else n[3] for m, d in zip(n, s)]
-    return _Strides(s[0], s[1], s[2])
+    b, r, h, _ = t.stride()
+    if (b | r | h) & 7 or not (b and r and h):
+        b, r, h = (d if n > 1 else t.shape[3] for n, d in zip(t.shape, (b, r, h)))
+    return _Strides(b, r, h)
 
 
 def _spans_arg(spans, rows: int):
@@ -185,7 +188,7 @@ def span_backward(q, k, v, spans, causal: bool, scale: float, cap: float, slopes
         slopes = slopes.contiguous()
     with _on(q.device):
         rows = B * ((Sq + 63) // 64) * 64
-        scratch = torch.empty(rows * (8 * H + 8) + rows // 64 * 16, dtype=torch.uint8, device=q.device)
+        scratch = torch.empty(rows * (8 * H + 8) + rows // 32 * 16, dtype=torch.uint8, device=q.device)
         st = _strides(q), _strides(k), _strides(v), _strides(dout), _strides(dq), _strides(dk)
         at = [addressof(s) for s in st]
         check(native.lib().rb_span_bwd(native.dtype_code(q.dtype), ptr(q), ptr(k), ptr(v), at[0], at[1], at[2], ptr(spans), batch, ptr(slopes), ptr(o),
@@ -205,11 +208,13 @@ class _SpanAttnFn(torch.autograd.Function):
         return o
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
+        if torch.is_grad_enabled():                 # create_graph: the gradients would look like constants
+            raise RuntimeError("span attention has no second derivatives")
         q, k, v, spans, slopes, o, lse2 = ctx.saved_tensors
         causal, scale, cap = ctx.args
-        return (*span_backward(q, k, v, spans, causal, scale, cap, slopes, o, lse2, dout), None, None, None, None, None)
+        dq, dk, dv = span_backward(q, k, v, spans, causal, scale, cap, slopes, o, lse2, dout)
+        return dq, dk, dv, None, None, None, None, None
 
 
 # ---------------------------------------------------------------- plain math
