@@ -27,6 +27,8 @@ class GPTConfig:
     num_layers: int = 24
     ffn_dim: int = 8192
     activation: str = "gelu"
+    attn_cap: float = 0.0          # scores s become cap tanh(s / cap); 0: they stay
+    alibi: bool = False            # scores fall with the distance, in place of the positional embedding
 
     @staticmethod
     def from_dict(d: dict) -> "GPTConfig":
@@ -44,7 +46,7 @@ class GPTConfig:
     def num_params(self) -> int:
         d, f, v, s, l = self.d_model, self.ffn_dim, self.vocab_size, self.seq_len, self.num_layers
         per_block = 4 * d * d + 4 * d + 2 * d * f + f + d + 4 * d
-        return v * d + s * d + l * per_block + 2 * d + d * v
+        return v * d + (0 if self.alibi else s * d) + l * per_block + 2 * d + d * v
 
     def flops_per_token(self) -> float:
         """Training FLOPs per token (fwd + bwd = 3x forward): dense GEMMs plus causal attention."""
@@ -59,9 +61,9 @@ class GPT(Module):
         super().__init__()
         self.cfg = cfg
         self.token_emb = Embedding(cfg.vocab_size, cfg.d_model, device, dtype)
-        self.pos_emb = Embedding(cfg.seq_len, cfg.d_model, device, dtype)
+        self.pos_emb = None if cfg.alibi else Embedding(cfg.seq_len, cfg.d_model, device, dtype)
         self.blocks = nn.ModuleList([
-            TransformerBlock(cfg.d_model, cfg.num_heads, cfg.ffn_dim, cfg.activation, True, device, dtype)
+            TransformerBlock(cfg.d_model, cfg.num_heads, cfg.ffn_dim, cfg.activation, True, device, dtype, cfg.attn_cap, cfg.alibi)
             for _ in range(cfg.num_layers)])
         self.ln_final = LayerNorm(cfg.d_model, 1e-5, device, dtype)
         self.head = Linear(cfg.d_model, cfg.vocab_size, False, device, dtype)
@@ -76,15 +78,16 @@ class GPT(Module):
                 elif name.endswith("bias"):
                     p.zero_()
 
-    def hidden(self, idx: torch.Tensor) -> torch.Tensor:
-        x = self.token_emb(idx, self.pos_emb.weight)
+    def hidden(self, idx: torch.Tensor, spans: Optional[torch.Tensor] = None) -> torch.Tensor:
+        x = self.token_emb(idx, None if self.pos_emb is None else self.pos_emb.weight)
         for blk in self.blocks:
-            x = blk(x)
+            x = blk(x) if spans is None else blk(x, spans=spans)
         return self.ln_final(x)
 
-    def forward(self, idx: torch.Tensor, targets: Optional[torch.Tensor] = None):
-        """Returns logits ``[B, S, V]``, or the mean next-token loss when ``targets`` is given."""
-        x = self.hidden(idx)
+    def forward(self, idx: torch.Tensor, targets: Optional[torch.Tensor] = None, spans: Optional[torch.Tensor] = None):
+        """Returns logits ``[B, S, V]``, or the mean next-token loss when ``targets`` is given.  ``spans``: the tokens that each
+        one sees (``F.document_spans``: packed documents, prefixes, padding), in the causal mask's place."""
+        x = self.hidden(idx, spans)
         if targets is None:
             return self.head(x)
         return F.lm_head_loss(x, self.head.weight, targets)

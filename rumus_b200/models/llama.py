@@ -28,6 +28,8 @@ class LlamaConfig:
     ffn_dim: int = 11008
     rope_theta: float = 10000.0
     rms_eps: float = 1e-5
+    attn_cap: float = 0.0          # scores s become cap tanh(s / cap); 0: they stay
+    alibi: bool = False            # scores fall with the distance, in place of the rotation
 
     @staticmethod
     def from_dict(d: dict) -> "LlamaConfig":
@@ -93,14 +95,14 @@ class LlamaBlock(Module):
         super().__init__()
         self.ln1 = RMSNorm(cfg.d_model, cfg.rms_eps, device, dtype)
         self.attn = MultiheadAttention(cfg.d_model, cfg.num_heads, bias=False, causal=True,
-                                       num_kv_heads=cfg.num_kv_heads, rope_theta=cfg.rope_theta,
-                                       device=device, dtype=dtype)
+                                       num_kv_heads=cfg.num_kv_heads, rope_theta=None if cfg.alibi else cfg.rope_theta,
+                                       device=device, dtype=dtype, attn_cap=cfg.attn_cap, alibi=cfg.alibi)
         self.ln2 = RMSNorm(cfg.d_model, cfg.rms_eps, device, dtype)
         self.mlp = LlamaMLP(cfg.d_model, cfg.ffn_dim, device, dtype)
 
-    def forward(self, x):
+    def forward(self, x, spans=None):
         y, skip = F.norm_skip(x, self.ln1.weight, None, self.ln1.eps, rms=True)
-        h = self.attn(y, residual=skip)
+        h = self.attn(y, residual=skip, spans=spans)
         y2, skip2 = F.norm_skip(h, self.ln2.weight, None, self.ln2.eps, rms=True)
         return self.mlp(y2, residual=skip2)
 
@@ -121,14 +123,15 @@ class Llama(Module):
                 if p.dim() >= 2:
                     p.copy_((torch.randn(p.shape, generator=g) * std).to(p.dtype))
 
-    def hidden(self, idx):
+    def hidden(self, idx, spans: Optional[torch.Tensor] = None):
         x = self.token_emb(idx)
         for blk in self.blocks:
-            x = blk(x)
+            x = blk(x) if spans is None else blk(x, spans=spans)
         return self.ln_final(x)
 
-    def forward(self, idx, targets: Optional[torch.Tensor] = None):
-        x = self.hidden(idx)
+    def forward(self, idx, targets: Optional[torch.Tensor] = None, spans: Optional[torch.Tensor] = None):
+        """``spans``: the tokens that each one sees (``F.document_spans``), in the causal mask's place."""
+        x = self.hidden(idx, spans)
         if targets is None:
             return self.head(x)
         return F.lm_head_loss(x, self.head.weight, targets)

@@ -31,6 +31,8 @@ class ParallelLlamaBlock(Module):
         self.hd = cfg.d_model // cfg.num_heads
         self.h_local = cfg.num_heads // T
         self.hkv_local = cfg.num_kv_heads // T
+        # this rank's heads' part of the distance bias
+        self.slopes = F.distance_slopes(cfg.num_heads, device)[tp.rank * self.h_local:(tp.rank + 1) * self.h_local] if cfg.alibi else None
         qkv_out = (cfg.num_heads + 2 * cfg.num_kv_heads) * self.hd
         self.ln1 = RMSNorm(cfg.d_model, cfg.rms_eps, device, dtype)
         # per-rank column layout: [q heads of this rank | k heads | v heads]
@@ -51,10 +53,15 @@ class ParallelLlamaBlock(Module):
         # no stand-alone residual add in forward, none for the two gradients in backward
         y1, skip = F.norm_skip(x_local, self.ln1.weight, None, self.ln1.eps, rms=True)
         qkv = self.qkv(y1)                                      # [M, (H + 2Hkv) * hd] local heads
-        qkv = F.rope_qkv(qkv.view(batch, seq, -1), seq, H, Hkv, hd, self.cfg.rope_theta)
+        qkv = qkv.view(batch, seq, -1)
+        if not self.cfg.alibi:
+            qkv = F.rope_qkv(qkv, seq, H, Hkv, hd, self.cfg.rope_theta)
         q, k, v = qkv.split([H * hd, Hkv * hd, Hkv * hd], dim=-1)
-        o = F.flash_attention(q.view(batch, seq, H, hd), k.view(batch, seq, Hkv, hd),
-                              v.view(batch, seq, Hkv, hd), True)
+        q, k, v = q.view(batch, seq, H, hd), k.view(batch, seq, Hkv, hd), v.view(batch, seq, Hkv, hd)
+        if self.cfg.attn_cap > 0 or self.slopes is not None:
+            o = F.span_attention(q, k, v, cap=self.cfg.attn_cap, slopes=self.slopes)
+        else:
+            o = F.flash_attention(q, k, v, True)
         h = self.out_proj(o.reshape(batch * seq, H * hd), residual=skip)
         y2, skip2 = F.norm_skip(h, self.ln2.weight, None, self.ln2.eps, rms=True)
         return self.down(F.swiglu(self.gate_up(y2)), residual=skip2)

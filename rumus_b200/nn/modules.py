@@ -165,11 +165,14 @@ class MultiheadAttention(Module):
     Checkpoint keys are ``q_proj/k_proj/v_proj/out_proj .weight/.bias`` (``[in,out]``) as in
     the reference; internally q/k/v live in ONE ``[d, (H + 2*Hkv)*hd]`` parameter so the
     projection is a single GEMM whose output feeds FlashAttention through strided views.
+
+    ``attn_cap``: scores s become cap tanh(s / cap); ``alibi``: scores fall with the distance, by ``F.distance_slopes``.  ``forward``'s
+    ``spans`` (int32 ``[B, S, 2]``, see ``F.document_spans``) name the keys that each row sees, in the causal mask's place.
     """
 
     def __init__(self, d_model: int, num_heads: int, bias: bool = True, causal: bool = True,
                  num_kv_heads: Optional[int] = None, rope_theta: Optional[float] = None,
-                 device=None, dtype=None):
+                 device=None, dtype=None, attn_cap: float = 0.0, alibi: bool = False):
         super().__init__()
         assert d_model % num_heads == 0
         self.d_model, self.num_heads = d_model, num_heads
@@ -177,6 +180,8 @@ class MultiheadAttention(Module):
         self.head_dim = d_model // num_heads
         self.causal = causal
         self.rope_theta = rope_theta
+        self.attn_cap, self.alibi = attn_cap, alibi
+        self._slopes = None
         bound = math.sqrt(1.0 / d_model)
         kv_dim = self.num_kv_heads * self.head_dim
         wq = _uniform((d_model, d_model), bound, _linear_rng, device, dtype)
@@ -195,12 +200,27 @@ class MultiheadAttention(Module):
         kv = self.num_kv_heads * self.head_dim
         return [self.d_model, kv, kv]
 
-    def forward(self, x, mask=None, residual=None):
+    def slopes(self, device) -> Optional[torch.Tensor]:
+        """The heads' slopes on ``device`` (constants, no part of the state), None without ``alibi``."""
+        if self.alibi and (self._slopes is None or self._slopes.device != device):
+            self._slopes = F.distance_slopes(self.num_heads, device)
+        return self._slopes if self.alibi else None
+
+    def forward(self, x, mask=None, residual=None, spans=None):
         B, S, _ = x.shape
         qkv = F.linear(x, self.qkv_weight, self.qkv_bias)
         H, Hkv, hd = self.num_heads, self.num_kv_heads, self.head_dim
         if self.rope_theta is not None:
+            if qkv.is_cuda and qkv.requires_grad:
+                qkv = qkv.clone()       # the rotation works in place, which autograd does not allow on a view that a custom function returned
             qkv = F.rope_qkv(qkv, S, H, Hkv, hd, self.rope_theta)
+        if spans is not None or self.attn_cap > 0 or self.alibi:
+            if mask is not None:
+                raise ValueError("an additive mask does not go with spans, a cap or a distance bias")
+            q, k, v = qkv.split(self._splits(), dim=-1)
+            o = F.span_attention(q.view(B, S, H, hd), k.view(B, S, Hkv, hd), v.view(B, S, Hkv, hd), spans,
+                                 self.causal and spans is None, cap=self.attn_cap, slopes=self.slopes(qkv.device))
+            return self.out_proj(o.reshape(B, S, self.d_model), residual=residual)
         if (mask is None and hd == 128 and qkv.is_cuda
                 and qkv.dtype in (torch.bfloat16, torch.float16) and qkv.data_ptr() % 16 == 0):
             # packed path: the backward kernels write d_q / d_k / d_v into one d_qkv buffer
@@ -262,22 +282,22 @@ class TransformerBlock(Module):
     """
 
     def __init__(self, d_model: int, num_heads: int, mlp_dim: Optional[int] = None,
-                 activation: str = "gelu", causal: bool = True, device=None, dtype=None):
+                 activation: str = "gelu", causal: bool = True, device=None, dtype=None, attn_cap: float = 0.0, alibi: bool = False):
         super().__init__()
         mlp_dim = mlp_dim or 4 * d_model
         self.d_model = d_model
         self.activation = activation
         self.ln1 = LayerNorm(d_model, 1e-5, device, dtype)
-        self.attn = MultiheadAttention(d_model, num_heads, True, causal, device=device, dtype=dtype)
+        self.attn = MultiheadAttention(d_model, num_heads, True, causal, device=device, dtype=dtype, attn_cap=attn_cap, alibi=alibi)
         self.ln2 = LayerNorm(d_model, 1e-5, device, dtype)
         self.mlp_fc1 = Linear(d_model, mlp_dim, True, device, dtype)
         self.mlp_fc2 = Linear(mlp_dim, d_model, True, device, dtype)
 
-    def forward(self, x, mask=None):
+    def forward(self, x, mask=None, spans=None):
         # the skip stream is taken from the norm op (see F.norm_skip): the gradient that comes back
         # along it is added inside the norm's backward kernel
         y, skip = F.norm_skip(x, self.ln1.weight, self.ln1.bias, self.ln1.eps)
-        h = self.attn(y, mask, residual=skip)
+        h = self.attn(y, mask, residual=skip, spans=spans)
         y2, skip2 = F.norm_skip(h, self.ln2.weight, self.ln2.bias, self.ln2.eps)
         return F.mlp(y2, self.mlp_fc1.weight, self.mlp_fc1.bias, self.mlp_fc2.weight,
                      self.mlp_fc2.bias, act=self.activation, residual=skip2)

@@ -691,6 +691,12 @@ def document_spans(documents, prefix=None, causal: bool = True):
     return _spans(documents, prefix, causal)
 
 
+def distance_slopes(heads: int, device=None):
+    """Slopes of a linear distance bias for ``span_attention``; see ``ops/span.py``."""
+    from .span import distance_slopes as _slopes
+    return _slopes(heads, device)
+
+
 def _sdpa_composed(q, k, v, causal, scale):
     """fp32 CUDA tensors: batched matmul + softmax kernels (the reference's composition,
     rumus/src/nn/attention.rs:17-58)."""

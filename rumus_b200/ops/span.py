@@ -142,8 +142,9 @@ def _spans_arg(spans, rows: int):
 
 # ---------------------------------------------------------------- kernels
 def span_forward(q, k, v, spans, causal: bool, scale: float, cap: float, slopes, out=None, lse: bool = True):
-    """Heads ``[B, Sq, H, D]`` and, with ``lse``, the rows' log-sum-exp in units of log 2 ``[B, H, Sq]``.  q, k, v: views that ``_view`` returns.
-    ``out``: contiguous tensor to write into."""
+    """Heads ``[B, Sq, H, D]`` and, with ``lse``, the rows' log-sum-exp in units of log 2 ``[B, H, Sq]``.  For heads that ``kernels_take``.  ``out``:
+    contiguous tensor to write into."""
+    q, k, v = _view(q), _view(k), _view(v)
     B, Sq, H, D = q.shape
     Sk, Hkv = k.shape[1], k.shape[2]
     if out is None:
@@ -268,7 +269,7 @@ def span_attention(q, k, v, spans=None, causal: bool = True, scale: Optional[flo
         raise TypeError(f"span attention on a GPU takes bfloat16 or float16 heads of a multiple of 8 numbers up to 128, not {q.dtype} of {q.shape[-1]}")
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _SpanAttnFn.apply(q, k, v, spans, bool(causal), scale, cap, slopes)
-    return span_forward(_view(q), _view(k), _view(v), spans, bool(causal), scale, cap, slopes, lse=False)[0]
+    return span_forward(q, k, v, spans, bool(causal), scale, cap, slopes, lse=False)[0]
 
 
 def span_decode(q, k_cache, v_cache, block_tables, ctx_lens, max_ctx: int, scale: Optional[float] = None, cap: float = 0.0, slopes=None, starts=None,

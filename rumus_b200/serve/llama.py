@@ -14,7 +14,7 @@ from typing import List
 import torch
 
 from ..nn.quant import QuantizedTensor, qmatmul_int4
-from ..ops import attention, functional as F, native
+from ..ops import attention, functional as F, native, span
 from ..ops._lib import check, count_launch, ptr, stream_ptr
 from .batch import StepBatch
 from .cache import PagedKVCache
@@ -98,6 +98,9 @@ class Int4LlamaShard:
         hd = m.d_model // m.num_heads
         self.hd = hd
         self.h_local, self.hkv_local = m.num_heads // world, m.num_kv_heads // world
+        # this rank's heads' part of the distance bias
+        self.slopes = F.distance_slopes(m.num_heads, device)[rank * self.h_local:(rank + 1) * self.h_local].contiguous() if m.alibi else None
+        self.shaped = m.attn_cap > 0 or m.alibi       # scores are capped or fall with the distance
         # row-parallel K splits must fall on quantisation-group boundaries: the FFN width is padded with
         # zero columns (gate, up) / zero rows (down) to a multiple of world x group size, which leaves the
         # function unchanged (silu(0) * 0 = 0 meets zero rows).  Llama-7B: 11008 -> 11264 at 4 and 8 ranks.
@@ -175,7 +178,9 @@ class Int4LlamaShard:
             q = qkv[:, : H * hd]
             k = qkv[:, H * hd: (H + Hkv) * hd]
             v = qkv[:, (H + Hkv) * hd:]
-            if fused:
+            if m.alibi:
+                cache.append(li, k, v, batch.slots)
+            elif fused:
                 cache.rope_append(li, qkv, H, batch.positions, batch.slots, m.rope_theta)
             else:
                 _rope(q, batch.positions, H, hd, m.rope_theta)
@@ -191,6 +196,8 @@ class Int4LlamaShard:
     def _attend(self, li, q, k, v, batch: StepBatch, cache: PagedKVCache, scale: float):
         """Single tokens through the paged decode kernel; each prompt portion through FlashAttention, whole
         prompts on the keys just computed, continuations on the prefix gathered from the cache."""
+        if self.shaped:
+            return self._attend_shaped(li, q, k, v, batch, cache, scale)
         if q.is_cuda:
             T, H, D = q.shape
             out = torch.empty((T, H, D), dtype=q.dtype, device=q.device)
@@ -214,6 +221,24 @@ class Int4LlamaShard:
             else:
                 outs.append(F.flash_attention(q[r][None], kk[None], vv[None], True, scale)[0])
         return out if q.is_cuda else outs[0] if len(outs) == 1 else torch.cat(outs)
+
+    def _attend_shaped(self, li, q, k, v, batch: StepBatch, cache: PagedKVCache, scale: float):
+        """The same with scores that are capped or fall with the distance."""
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        cap = self.cfg.model.attn_cap
+        if batch.n_rows:
+            span.span_decode(q[:batch.n_rows], cache.k[li], cache.v[li], batch.tables, batch.ctx, batch.max_ctx, scale, cap, self.slopes,
+                             head_major=cache.head_major, out=out[:batch.n_rows])
+        for i, s in enumerate(batch.segments):
+            r = slice(s.row0, s.row0 + s.n)
+            kk, vv = k[r], v[r]
+            if s.start:
+                kk, vv = cache.gather(li, batch.seg_tables[i].long(), torch.arange(s.start + s.n, device=q.device))
+            if q.is_cuda:
+                span.span_forward(q[r][None], kk[None], vv[None], None, True, scale, cap, self.slopes, out=out[r][None], lse=False)
+            else:
+                out[r] = span.span_attention(q[r][None], kk[None], vv[None], None, True, scale, cap, self.slopes)[0]
+        return out
 
     def logits(self, hidden: torch.Tensor) -> torch.Tensor:
         return native.gemm(hidden.contiguous(), self.head) if hidden.is_cuda else hidden @ self.head
