@@ -37,15 +37,20 @@ __device__ __forceinline__ void span_pack32(const uint32_t* f, uint32_t* w) {
 }
 
 // ---------------------------------------------------------------- dQ
-// A CTA owns 128 query rows of a head and goes over tiles of 64 keys; two warpgroups take the tiles in turn, a thread owns a row.  Q and dO lie in
-// tensor memory: as left operands from shared memory they would take most of its port (128 bytes a clock).
+// A CTA owns 128 query rows of a head and goes over tiles of 64 keys; two warpgroups take the tiles in turn, a thread owns a row.
+//
+// delta from the rounded O is off by 2^-9 of the row's gradient, which is more than dS itself where one key has nearly all the weight.  So the sweep takes
+// it as a first guess d0 only, sums delta = sum p dP in fp32 beside, and corrects the result: dQ = scale (sum g (dP - d0) K + (d0 - delta) sum g K) with
+// g = p (1 - t^2); sum g K is one product more, and the second kernel gets the exact delta.  (Gradients of bfloat16 heads with scores of deviation 4:
+// 1.2 % off without it, 0.24 % with it; the roundings of dS and of the result leave 0.23 %.)
 template <int HD>
 struct SpanDqCfg {
-  static constexpr int SUB = HD / 64, SUB_BYTES = 64 * 128, TILE = SUB * SUB_BYTES;
-  static constexpr int STAGES = HD == 128 ? 6 : 8, ROW_SUB = 128 * 128;      // 128 rows of Q, dO or O take as much as a stage: at first the last three hold them
-  static constexpr int SMEM_BYTES = STAGES * 2 * TILE + 1024 + 256;
-  static_assert(SUB * ROW_SUB == 2 * TILE, "rows in the place of a stage");
-  static constexpr int Q_COL = 0, DO_COL = 64, DQ_COL = 128, S_COL = 256, DP_COL = 384;     // S, dP of buffer w: + 64 w
+  static constexpr int SUB = HD / 64, KV_SUB = 64 * 128, TILE = SUB * KV_SUB;          // 64 keys
+  static constexpr int ROW_SUB = 128 * 128, ROWS = SUB * ROW_SUB;                       // 128 rows: as much as a stage's K and V
+  static constexpr int STAGES = HD == 128 ? 4 : 8;
+  static constexpr int SMEM_BYTES = 2 * ROWS + STAGES * 2 * TILE + 1024 + 256;
+  static_assert(ROWS == 2 * TILE, "O lies in the last stage at first");
+  static constexpr int DQ_COL = 0, GK_COL = 128, S_COL = 256, DP_COL = 384;     // S (then g and dS), dP of buffer w: + 64 w
 };
 
 template <typename T, int HD, bool CAP, bool BIAS>
@@ -55,14 +60,17 @@ __global__ void __launch_bounds__(320, 1)
                    const SpanBwdParams p) {
   using C = SpanDqCfg<HD>;
   extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::STAGES * 2 * C::TILE);       // [STAGES] {K, V}
+  uint8_t* sQ = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* sdO = sQ + C::ROWS;
+  uint8_t* ring = sdO + C::ROWS;                                 // [STAGES] {K, V}
+  uint8_t* sO = ring + (C::STAGES - 1) * 2 * C::TILE;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(ring + C::STAGES * 2 * C::TILE);
   uint64_t *full = bars, *empty = full + C::STAGES, *sdp_full = empty + C::STAGES, *ds_ready = sdp_full + 2, *dq_done = ds_ready + 2,
            *rows_full = dq_done + 1, *rows_read = rows_full + 1;
   uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(rows_read + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_ptr + 1);
   __shared__ int4 s_range[4];
-  __shared__ float s_delta[128];
+  __shared__ float s_sum[2][2][128];                             // [first guess, sum][warpgroup]
 
   const int warp = uniform_warp_idx(), lane = threadIdx.x & 31;
   int tile, unit;
@@ -90,13 +98,12 @@ __global__ void __launch_bounds__(320, 1)
     fence_barrier_init();
     fence_proxy_async();
     // this thread's own barriers: the copies need no one else
-    mbar_arrive_expect_tx(smem_u32(rows_full), 3 * 2 * C::TILE);
-    uint8_t* rows = smem + (C::STAGES - 3) * 2 * C::TILE;
+    mbar_arrive_expect_tx(smem_u32(rows_full), 3 * C::ROWS);
 #pragma unroll
     for (int s = 0; s < C::SUB; ++s) {
-      tma_load_4d(smem_u32(rows + s * C::ROW_SUB), &tq, smem_u32(rows_full), s * 64, q0, h, b);
-      tma_load_4d(smem_u32(rows + 2 * C::TILE + s * C::ROW_SUB), &tdo, smem_u32(rows_full), s * 64, q0, h, b);
-      tma_load_4d(smem_u32(rows + 4 * C::TILE + s * C::ROW_SUB), &to, smem_u32(rows_full), s * 64, q0, h, b);
+      tma_load_4d(smem_u32(sQ + s * C::ROW_SUB), &tq, smem_u32(rows_full), s * 64, q0, h, b);
+      tma_load_4d(smem_u32(sdO + s * C::ROW_SUB), &tdo, smem_u32(rows_full), s * 64, q0, h, b);
+      tma_load_4d(smem_u32(sO + s * C::ROW_SUB), &to, smem_u32(rows_full), s * 64, q0, h, b);
     }
   }
   int2 span = make_int2(0, 0);
@@ -114,60 +121,7 @@ __global__ void __launch_bounds__(320, 1)
   const uint32_t tmem_base = *tmem_ptr;
   const int4 all = span_range_join(span_range_join(s_range[0], s_range[1]), span_range_join(s_range[2], s_range[3]));
   const int j0 = all.x < all.y ? all.x / 64 : 0, n = all.x < all.y ? (all.y + 63) / 64 - j0 : 0;
-
-  const uint32_t lane_addr = tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-  float lse2 = 0.f;
   bool ok = true;
-  if (warp < 8) {
-    // Q (first warpgroup) and dO (second) into tensor memory; delta on the way.  By way of shared memory: a thread's own row of loads, 16 bytes of a line
-    // each, took 10000 cycles.
-    ok = mbar_wait(smem_u32(rows_full), 0, abort_flag, p.status, RB_ERR_TIMEOUT_FULL);
-    ok = __all_sync(0xffffffffu, ok);
-    const uint8_t* from = smem + (C::STAGES - 3 + wg) * 2 * C::TILE + t * 128;
-    const uint8_t* o = smem + (C::STAGES - 1) * 2 * C::TILE + t * 128;
-    float delta = 0.f;
-#pragma unroll
-    for (int c = 0; c < HD / 32; ++c) {
-      uint32_t w[16];
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int d = c * 32 + g * 8, at = (d >> 6) * C::ROW_SUB + ((((d >> 3) & 7) ^ (t & 7)) << 4);
-        const uint4 v = *reinterpret_cast<const uint4*>(from + at);
-        w[g * 4] = v.x; w[g * 4 + 1] = v.y; w[g * 4 + 2] = v.z; w[g * 4 + 3] = v.w;
-        if (wg == 1) {
-          const uint4 y = *reinterpret_cast<const uint4*>(o + at);
-          const uint32_t z[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 e = unpack2<T>(w[g * 4 + i]), f = unpack2<T>(z[i]);
-            delta = fmaf(e.x, f.x, fmaf(e.y, f.y, delta));
-          }
-        }
-      }
-      tmem_st_32x32b_x16(lane_addr + (wg == 0 ? C::Q_COL : C::DO_COL) + c * 16, w);
-    }
-    mbar_arrive(smem_u32(rows_read));
-    if (live && span.x < span.y) lse2 = p.lse2[(static_cast<long long>(b) * p.H + h) * p.Sq + row];
-    if (row < p.sq_pad) {
-      const long long at = (static_cast<long long>(b) * p.H + h) * p.sq_pad + row;
-      if (wg == 0) p.row_lse2[at] = -lse2;
-      else p.row_delta[at] = -delta;
-      if (h == 0 && wg == 0) {
-        p.row_lo[static_cast<long long>(b) * p.sq_pad + row] = span.x;
-        p.row_hi[static_cast<long long>(b) * p.sq_pad + row] = span.y;
-        if (lane == 0) {
-          int4 r = s_range[warp];
-          if (row + 32 > p.Sq) r.w = 0;           // rows behind the last one see nothing: their scores are masked
-          p.range[(static_cast<long long>(b) * p.sq_pad + row) / 32] = r;
-        }
-      }
-    }
-    if (wg == 1) s_delta[t] = delta;
-    tmem_st_wait();
-  }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
 
   if (warp == 8) {
     // ------------------------------ TMA producer ------------------------------
@@ -175,15 +129,15 @@ __global__ void __launch_bounds__(320, 1)
       int st = 0;
       uint32_t ph = 0;
       for (int i = 0; i < n; ++i) {
-        ok = i == C::STAGES - 3 ? mbar_wait(smem_u32(rows_read), 0, abort_flag, p.status, RB_ERR_TIMEOUT_EMPTY)
+        ok = i == C::STAGES - 1 ? mbar_wait(smem_u32(rows_read), 0, abort_flag, p.status, RB_ERR_TIMEOUT_EMPTY)
                                 : mbar_wait(smem_u32(&empty[st]), ph ^ 1, abort_flag, p.status, RB_ERR_TIMEOUT_EMPTY);
         if (!ok) break;
-        const uint32_t bar = smem_u32(&full[st]), dst = smem_u32(smem + st * 2 * C::TILE);
+        const uint32_t bar = smem_u32(&full[st]), dst = smem_u32(ring + st * 2 * C::TILE);
         mbar_arrive_expect_tx(bar, 2 * C::TILE);
 #pragma unroll
         for (int s = 0; s < C::SUB; ++s) {
-          tma_load_4d(dst + s * C::SUB_BYTES, &tk, bar, s * 64, (j0 + i) * 64, hkv, b);
-          tma_load_4d(dst + C::TILE + s * C::SUB_BYTES, &tv, bar, s * 64, (j0 + i) * 64, hkv, b);
+          tma_load_4d(dst + s * C::KV_SUB, &tk, bar, s * 64, (j0 + i) * 64, hkv, b);
+          tma_load_4d(dst + C::TILE + s * C::KV_SUB, &tv, bar, s * 64, (j0 + i) * 64, hkv, b);
         }
         if (++st == C::STAGES) { st = 0; ph ^= 1; }
       }
@@ -194,29 +148,33 @@ __global__ void __launch_bounds__(320, 1)
     // ------------------------------ MMA issuer --------------------------------
     constexpr uint32_t idesc_s = make_idesc(UmmaFormat<T>::value, 0, 0, 128, 64);
     constexpr uint32_t idesc_q = make_idesc(UmmaFormat<T>::value, 0, 1, 128, HD);
+    const uint64_t qd = make_smem_desc_sw128(smem_u32(sQ), 16, 1024), dod = make_smem_desc_sw128(smem_u32(sdO), 16, 1024);
     int st_in = 0, st_out = 0;
     uint32_t ph_in = 0;
     auto issue = [&](int i) {            // S and dP of tile i, the next stage
       ok = mbar_wait(smem_u32(&full[st_in]), ph_in, abort_flag, p.status, RB_ERR_TIMEOUT_FULL);
       if (!ok) return;
       tc_fence_after();
-      const uint32_t k = smem_u32(smem + st_in * 2 * C::TILE);
+      const uint32_t k = smem_u32(ring + st_in * 2 * C::TILE);
       const uint64_t kd = make_smem_desc_sw128(k, 16, 1024), vd = make_smem_desc_sw128(k + C::TILE, 16, 1024);
 #pragma unroll
       for (int s = 0; s < C::SUB; ++s) {
-        umma_f16_ts_w4<8, 2>(tmem_base + C::S_COL + (i & 1) * 64, tmem_base + C::Q_COL + s * 32, kd + s * (C::SUB_BYTES >> 4), idesc_s, s != 0);
-        umma_f16_ts_w4<8, 2>(tmem_base + C::DP_COL + (i & 1) * 64, tmem_base + C::DO_COL + s * 32, vd + s * (C::SUB_BYTES >> 4), idesc_s, s != 0);
+        umma_f16_w4<2, 2>(tmem_base + C::S_COL + (i & 1) * 64, qd + s * (C::ROW_SUB >> 4), kd + s * (C::KV_SUB >> 4), idesc_s, s != 0);
+        umma_f16_w4<2, 2>(tmem_base + C::DP_COL + (i & 1) * 64, dod + s * (C::ROW_SUB >> 4), vd + s * (C::KV_SUB >> 4), idesc_s, s != 0);
       }
       umma_commit_w(smem_u32(&sdp_full[i & 1]));
       if (++st_in == C::STAGES) { st_in = 0; ph_in ^= 1; }
     };
+    if (n > 0) ok = mbar_wait(smem_u32(rows_full), 0, abort_flag, p.status, RB_ERR_TIMEOUT_FULL);
     for (int i = 0; i < 2 && i < n && ok; ++i) issue(i);
     for (int i = 0; i < n && ok; ++i) {
       ok = mbar_wait(smem_u32(&ds_ready[i & 1]), (i >> 1) & 1, abort_flag, p.status, RB_ERR_TIMEOUT_FLAG);
       if (!ok) break;
       tc_fence_after();
-      const uint64_t kd = make_smem_desc_sw128(smem_u32(smem + st_out * 2 * C::TILE), C::SUB_BYTES, 1024);
-      umma_f16_ts_w4<8, 128>(tmem_base + C::DQ_COL, tmem_base + C::S_COL + (i & 1) * 64, kd, idesc_q, i != 0);
+      const uint64_t kd = make_smem_desc_sw128(smem_u32(ring + st_out * 2 * C::TILE), C::KV_SUB, 1024);
+      const uint32_t g = tmem_base + C::S_COL + (i & 1) * 64;
+      umma_f16_ts_w4<8, 128>(tmem_base + C::GK_COL, g, kd, idesc_q, i != 0);
+      umma_f16_ts_w4<8, 128>(tmem_base + C::DQ_COL, g + 32, kd, idesc_q, i != 0);
       umma_commit_w(smem_u32(&empty[st_out]));
       if (i + 1 == n) umma_commit_w(smem_u32(dq_done));
       if (++st_out == C::STAGES) st_out = 0;
@@ -224,8 +182,43 @@ __global__ void __launch_bounds__(320, 1)
     }
   } else {
     // ------------------------------ softmax warpgroups ------------------------
-    const float slope2 = BIAS ? p.c.slopes[h] * kLog2e : 0.f, delta = s_delta[t];
+    const uint32_t lane_addr = tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    const float slope2 = BIAS ? p.c.slopes[h] * kLog2e : 0.f;
     const uint32_t s_addr = lane_addr + C::S_COL + wg * 64, dp_addr = lane_addr + C::DP_COL + wg * 64;
+    const float lse2 = live && span.x < span.y ? p.lse2[(static_cast<long long>(b) * p.H + h) * p.Sq + row] : 0.f;
+    const long long at = (static_cast<long long>(b) * p.H + h) * p.sq_pad + row;
+    if (wg == 0 && row < p.sq_pad) {
+      p.row_lse2[at] = -lse2;
+      if (h == 0) {
+        p.row_lo[static_cast<long long>(b) * p.sq_pad + row] = span.x;
+        p.row_hi[static_cast<long long>(b) * p.sq_pad + row] = span.y;
+        if (lane == 0) {
+          int4 r = s_range[warp];
+          if (row + 32 > p.Sq) r.w = 0;           // rows behind the last one see nothing: their scores are masked
+          p.range[(static_cast<long long>(b) * p.sq_pad + row) / 32] = r;
+        }
+      }
+    }
+    // first guess of delta: dO.O, half of the columns each.  By way of shared memory: a thread's own row of loads, 16 bytes of a line each, took 10000 cycles.
+    ok = mbar_wait(smem_u32(rows_full), 0, abort_flag, p.status, RB_ERR_TIMEOUT_FULL);
+    ok = __all_sync(0xffffffffu, ok);
+    float guess = 0.f;
+#pragma unroll
+    for (int c = 0; c < HD / 16; ++c) {
+      const int d = wg * (HD / 2) + c * 8, in = t * 128 + (d >> 6) * C::ROW_SUB + ((((d >> 3) & 7) ^ (t & 7)) << 4);
+      const uint4 v = *reinterpret_cast<const uint4*>(sdO + in), y = *reinterpret_cast<const uint4*>(sO + in);
+      const uint32_t e4[4] = {v.x, v.y, v.z, v.w}, f4[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 e = unpack2<T>(e4[i]), f = unpack2<T>(f4[i]);
+        guess = fmaf(e.x, f.x, fmaf(e.y, f.y, guess));
+      }
+    }
+    mbar_arrive(smem_u32(rows_read));
+    s_sum[0][wg][t] = guess;
+    asm volatile("bar.sync 1, 256;" ::: "memory");          // the softmax warps, also where a wait ran out
+    guess = s_sum[0][0][t] + s_sum[0][1][t];
+    uint64_t sum2 = 0;                                       // sum p dP of this warpgroup's tiles
     for (int i = wg; i < n && ok; i += 2) {
       ok = mbar_wait(smem_u32(&sdp_full[wg]), (i >> 1) & 1, abort_flag, p.status, RB_ERR_TIMEOUT_TMEM_FULL);
       ok = __all_sync(0xffffffffu, ok);
@@ -235,16 +228,19 @@ __global__ void __launch_bounds__(320, 1)
       const bool masked = kv0 < all.z || kv0 + 64 > all.w;
       const int side = !BIAS ? 1 : p.c.causal || q0 + off >= kv0 + 63 ? 1 : q0 + 127 + off <= kv0 ? -1 : 0;
       const float slope = side > 0 ? slope2 : -slope2;
-      const uint64_t minus = both(-delta);
-      uint32_t ds[2][16];
-      // dS of chunk c of 32 keys; PART: some of them are unseen
+      const uint64_t minus = both(-guess);
+      uint32_t g[2][16], ds[2][16];
+      // g and dS of chunk c of 32 keys; PART: some of them are unseen
       auto chunk = [&](int c, auto part, uint32_t seen) {
         constexpr bool PART = decltype(part)::value;
         uint32_t s[32], dp[32], slip[32];
         tmem_ld_32x32b_x32(s_addr + c * 32, s);
         tmem_ld_32x32b_x32(dp_addr + c * 32, dp);
         tmem_ld_wait();
-        if (PART) span_mask32(s, seen, 0);           // what unseen keys hold decides nothing
+        if (PART) {                                          // what unseen keys hold decides nothing
+          span_mask32(s, seen, 0);
+          span_mask32(dp, seen, 0);
+        }
         const float first = (float)(row + off - kv0 - c * 32), reach = CAP ? span_reach32(s) : 0.f;
         if (BIAS && side != 0) {
           span_score32<CAP, true>(s, p.c, SpanAdd<true, false>({fmaf(-slope, first, -lse2), slope}, nullptr), slip, reach);
@@ -252,14 +248,17 @@ __global__ void __launch_bounds__(320, 1)
           span_score32<CAP, true>(s, p.c, SpanAdd<false, false>({-lse2, 0.f}, nullptr), slip, reach);
           if constexpr (BIAS) span_both_sides32<-1>(s, slope2, first);
         }
+        if (PART) span_mask32(s, seen, 0xff800000u);
 #pragma unroll
         for (int k = 0; k < 32; k += 2) {
           uint64_t w = f32x2(fast_exp2(__uint_as_float(s[k])), fast_exp2(__uint_as_float(s[k + 1])));
+          const uint64_t d = pair_at(dp, k);
+          sum2 = fma_f32x2(w, d, sum2);
           if (CAP) w = mul_f32x2(w, pair_at(slip, k));
-          set_pair(s, k, mul_f32x2(w, add_f32x2(pair_at(dp, k), minus)));
+          const float2 a = f32x2_get(w), e = f32x2_get(mul_f32x2(w, add_f32x2(d, minus)));
+          g[c][k / 2] = pack2<T>(a.x, a.y);
+          ds[c][k / 2] = pack2<T>(e.x, e.y);
         }
-        if (PART) span_mask32(s, seen, 0);
-        span_pack32<T>(s, ds[c]);
       };
       if (!masked) {
         chunk(0, std::false_type{}, 0xffffffffu);
@@ -271,53 +270,66 @@ __global__ void __launch_bounds__(320, 1)
           const uint32_t seen = span_bits(span.x - kv0 - c * 32, span.y - kv0 - c * 32);
           if (__all_sync(0xffffffffu, seen == 0)) {
 #pragma unroll
-            for (int k = 0; k < 16; ++k) ds[c][k] = 0;
+            for (int k = 0; k < 16; ++k) g[c][k] = ds[c][k] = 0;
           } else {
             chunk(c, std::true_type{}, seen);
           }
         }
       }
-      tmem_st_32x32b_x16(s_addr, ds[0]);
-      tmem_st_32x32b_x16(s_addr + 16, ds[1]);
+      tmem_st_32x32b_x16(s_addr, g[0]);
+      tmem_st_32x32b_x16(s_addr + 16, g[1]);
+      tmem_st_32x32b_x16(s_addr + 32, ds[0]);
+      tmem_st_32x32b_x16(s_addr + 48, ds[1]);
       tmem_st_wait();
       tc_fence_before();
       mbar_arrive(smem_u32(&ds_ready[wg]));
     }
+    const float2 part = f32x2_get(sum2);
+    s_sum[1][wg][t] = part.x + part.y;
+    asm volatile("bar.sync 1, 256;" ::: "memory");
+    const float delta = s_sum[1][0][t] + s_sum[1][1][t];
+    if (wg == 1 && row < p.sq_pad) p.row_delta[at] = -delta;
     if (ok && n > 0) {
       ok = mbar_wait(smem_u32(dq_done), 0, abort_flag, p.status, RB_ERR_TIMEOUT_TMEM_EMPTY);
       ok = __all_sync(0xffffffffu, ok);
       tc_fence_after();
     }
     if (ok) {
-      // warpgroup w takes columns [w HD / 2, (w + 1) HD / 2): through shared memory (all copies have landed and been used), from there in whole rows
-      uint8_t* stage = smem + t * 128;
+      // warpgroup w takes columns [w HD / 2, (w + 1) HD / 2): through shared memory, in the place of Q, and from there in whole rows
+      const float slipped = guess - delta;
+      uint8_t* stage = sQ + t * 128;
 #pragma unroll 1
       for (int c = 0; c < HD / 64; ++c) {
         const int d0 = wg * (HD / 2) + c * 32;
-        uint32_t r[32];
+        uint32_t r[32], k32[32];
         if (n > 0) {
           tmem_ld_32x32b_x32(lane_addr + C::DQ_COL + d0, r);
+          tmem_ld_32x32b_x32(lane_addr + C::GK_COL + d0, k32);
           tmem_ld_wait();
         } else {
 #pragma unroll
-          for (int k = 0; k < 32; ++k) r[k] = 0;
+          for (int k = 0; k < 32; ++k) r[k] = k32[k] = 0;
         }
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           const int d = d0 + g * 8;
           uint32_t w[4];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) w[k] = pack2<T>(__uint_as_float(r[g * 8 + 2 * k]) * p.grad_scale, __uint_as_float(r[g * 8 + 2 * k + 1]) * p.grad_scale);
+          for (int k = 0; k < 4; ++k) {
+            const int i = g * 8 + 2 * k;
+            w[k] = pack2<T>(fmaf(slipped, __uint_as_float(k32[i]), __uint_as_float(r[i])) * p.grad_scale,
+                            fmaf(slipped, __uint_as_float(k32[i + 1]), __uint_as_float(r[i + 1])) * p.grad_scale);
+          }
           *reinterpret_cast<uint4*>(stage + (d >> 6) * C::ROW_SUB + ((((d >> 3) & 7) ^ (t & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
         }
       }
     }
     fence_proxy_async_smem();
-    asm volatile("bar.sync 1, 256;" ::: "memory");          // the softmax warps, also where a wait ran out
+    asm volatile("bar.sync 1, 256;" ::: "memory");
     if (threadIdx.x == 0 && ok) {
 #pragma unroll
       for (int s = 0; s < C::SUB; ++s)
-        if (s * 64 < p.D) tma_store_4d(&tdq, smem_u32(smem + s * C::ROW_SUB), s * 64, q0, h, b);
+        if (s * 64 < p.D) tma_store_4d(&tdq, smem_u32(sQ + s * C::ROW_SUB), s * 64, q0, h, b);
       tma_store_commit();
       tma_store_wait_read<0>();
     }

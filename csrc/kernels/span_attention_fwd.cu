@@ -216,12 +216,12 @@ __global__ void __launch_bounds__(SpanFwdCfg<HD>::THREADS, 1)
     const int begin = x ? first[1] : first[0], end = x ? last[1] : last[0];
     const int lo_max = x ? lo_all[1] : lo_all[0], hi_min = x ? hi_all[1] : hi_all[0];
     const float slope2 = BIAS ? p.c.slopes[h] * kLog2e : 0.f;
-    // Weights are relative to `ref`, which follows the row's maximum only when that may be far away: a tile's weights are made in one pass over its
-    // scores, without their maximum (the second half's scores, on the FMA pipe, between the first one's exponentials, on the special-function
-    // pipe).  Where the largest product says that the reference may be no good, the tile is done again in two passes.
-    // How far from its reference a weight may be: fp16 ones go up to 2^16, and small ones lose bits below 2^-14; bf16 has the range of fp32.
-    // (Not all of it: what a value of 2^90 times a weight of 2^30 is still has to be a number.)  LEAST: of a first tile's sum.
-    constexpr float UP = UmmaFormat<T>::value == 1 ? 30.f : 15.f, LEAST = UmmaFormat<T>::value == 1 ? 1.f / (1 << 30) : 1.f / (1 << 8);
+    // Weights are relative to `ref`: a row's largest score in the first tile that it sees, where two passes look for it (the weight of a key that has nearly
+    // all of it is then 1, and rounds to itself).  After that `ref` follows the maximum only when that may be far away, and a tile's weights are made in
+    // one pass over its scores, without their maximum.  Where the largest product says that the reference may be no good, two passes do the tile again.
+    // UP: how far above its reference a weight may be.  fp16 goes up to 2^16; bf16 has the range of fp32, but what a value of 2^90 times a weight of
+    // 2^30 is still has to be a number.
+    constexpr float UP = UmmaFormat<T>::value == 1 ? 30.f : 15.f;
     float ref = 0.f, l = 0.f;
     bool fresh = true, ok = true;                       // fresh: the row has seen no key yet
     bool flat = false, slow = false;                    // what the last tile needed: the general tanh, the two passes
@@ -275,7 +275,7 @@ __global__ void __launch_bounds__(SpanFwdCfg<HD>::THREADS, 1)
       };
       const bool sees = span.x < min(kv0 + C::BN, span.y) && span.y > max(kv0, span.x);
       bool done = false;
-      if (!slow) {
+      if (!slow && !__any_sync(0xffffffffu, fresh && sees)) {
         uint32_t packed[2][16];
         float sum = 0.f;
         bool quick = !masked && side != 0 && !(CAP && flat);
@@ -339,10 +339,9 @@ __global__ void __launch_bounds__(SpanFwdCfg<HD>::THREADS, 1)
         float most = reach * fabsf(p.c.scale2);
         if (CAP) most = fminf(most, p.c.out2);
         if (BIAS && slope2 < 0.f) most = fmaf(-slope2, (float)max(abs(away), abs(away - C::BN + 1)), most);
-        done = __all_sync(0xffffffffu, most - ref <= UP && (!fresh || !sees || sum >= LEAST));
+        done = __all_sync(0xffffffffu, most - ref <= UP);
         if (done) {
           l += sum;
-          fresh = fresh && !sees;
           tmem_st_32x32b_x16(s_addr, packed[0]);
           tmem_st_32x32b_x16(s_addr + 16, packed[1]);
         }
@@ -350,12 +349,28 @@ __global__ void __launch_bounds__(SpanFwdCfg<HD>::THREADS, 1)
       if (!done) {
         float mx = -INFINITY;
         reach = 0.f;
+        if constexpr (BIAS) {
 #pragma unroll 1
-        for (int c = 0; c < 2; ++c) {
-          uint32_t s[32];
-          if (!scores(c, 0.f, s)) continue;
+          for (int c = 0; c < 2; ++c) {
+            uint32_t s[32];
+            if (!scores(c, 0.f, s)) continue;
 #pragma unroll
-          for (int k = 0; k < 32; ++k) mx = fmaxf(mx, __uint_as_float(s[k]));
+            for (int k = 0; k < 32; ++k) mx = fmaxf(mx, __uint_as_float(s[k]));
+          }
+        } else {
+          // scores rise with the products (fall, where the scale is below zero): the score of the largest is the largest
+          const uint32_t flip = p.c.scale2 < 0.f ? 0x80000000u : 0u;
+#pragma unroll 1
+          for (int c = 0; c < 2; ++c) {
+            uint32_t s[32];
+            tmem_ld_32x32b_x32(s_addr + c * 32, s);
+            tmem_ld_wait();
+            const uint32_t seen = masked ? span_bits(span.x - kv0 - c * 32, span.y - kv0 - c * 32) : 0xffffffffu;
+#pragma unroll
+            for (int k = 0; k < 32; ++k)
+              if (seen >> k & 1) mx = fmaxf(mx, __uint_as_float(s[k] ^ flip));
+          }
+          if (mx > -INFINITY) mx = CAP ? fabsf(p.c.out2) * tanhf(fabsf(p.c.in) * mx) : fabsf(p.c.scale2) * mx;
         }
         // a maximum that goes on rising is looked for at once in the next tile
         slow = !__all_sync(0xffffffffu, fresh || mx <= ref + UP);
