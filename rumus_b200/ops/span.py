@@ -5,7 +5,8 @@
     o_i = sum_j softmax(x_i)_j v_j                                         (zeros for a row that sees no key)
 
 Spans cover packed documents, prompts whose beginning is seen by all of it, windows and padding (``document_spans``).  On a GPU one kernel forward and
-two backward (``csrc/kernels/span_attention_{fwd,bwd}.cu``) and one for a new token over pages (``span_decode.cu``); on a CPU plain math.  Gradients are
+two backward (``csrc/kernels/span_attention_{fwd,bwd}.cu``; in 32 bits one each, ``span_attention_f32.cu``) and one for a new token over pages
+(``span_decode.cu``); on a CPU plain math.  Gradients are
 summed in a fixed order: the same inputs give the same gradients.
 """
 from __future__ import annotations
@@ -24,6 +25,8 @@ P, LL, I, Fl = c_void_p, c_longlong, c_int, c_float
 native.register_signature("rb_span_fwd_splits", [I, I, I, I])
 native.register_signature("rb_span_fwd", [I] + [P] * 7 + [LL] + [P] * 5 + [I] * 8 + [Fl, Fl, P])
 native.register_signature("rb_span_bwd", [I] + [P] * 7 + [LL] + [P] * 11 + [I] * 7 + [Fl, Fl, P])
+native.register_signature("rb_span_f32_fwd", [I] + [P] * 7 + [LL] + [P] * 3 + [I] * 6 + [Fl, Fl, P])
+native.register_signature("rb_span_f32_bwd", [I] + [P] * 7 + [LL] + [P] * 8 + [I] * 6 + [Fl, Fl, P])
 native.register_signature("rb_span_decode_splits", [I, I, I, I])
 native.register_signature("rb_span_decode", [I, I, P, LL, LL] + [P] * 9 + [I] * 8 + [Fl, Fl, P])
 
@@ -98,7 +101,7 @@ def _rows_ok(q, k, v, spans, scale, cap, slopes) -> None:
 
 
 def kernels_take(q: torch.Tensor) -> bool:
-    """Whether the GPU kernels cover heads of this type and size."""
+    """Whether the 16-bit GPU kernels cover heads of this type and size."""
     return q.dtype in HALVES and q.shape[-1] % 8 == 0 and 0 < q.shape[-1] <= 128
 
 
@@ -117,9 +120,9 @@ def _view(t: torch.Tensor) -> torch.Tensor:
     """The view itself if the kernels read it in place (rows of neighbouring numbers, 16-byte aligned, no dimension that repeats), else a copy."""
     b, r, h, one = t.stride()
     if one == 1 and t.data_ptr() % 16 == 0:
-        if not (b | r | h) & 7 and 0 < b < 2 ** 39 and 0 < r < 2 ** 39 and 0 < h < 2 ** 39:
+        if not (b | r | h) & 7 and 0 < b < 2 ** 38 and 0 < r < 2 ** 38 and 0 < h < 2 ** 38:
             return t
-        if all(n == 1 or (d > 0 and d % 8 == 0 and d < 2 ** 39) for n, d in zip(t.shape, (b, r, h))):
+        if all(n == 1 or (d > 0 and d % 8 == 0 and d < 2 ** 38) for n, d in zip(t.shape, (b, r, h))):
             return t
     return t.clone(memory_format=torch.contiguous_format)
 
@@ -218,6 +221,61 @@ class _SpanAttnFn(torch.autograd.Function):
         return dq, dk, dv, None, None, None, None, None
 
 
+class _SpanF32Fn(torch.autograd.Function):
+    """Heads of 16, 32, 64 or 128 numbers in 32 bits."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, spans, causal, scale, cap, slopes):
+        q, k, v = _view(q), _view(k), _view(v)
+        B, Sq, H, D = q.shape
+        Sk, Hkv = k.shape[1], k.shape[2]
+        o, lse = q.new_empty(q.shape), q.new_empty((B, H, Sq))
+        ctx.args = causal, scale, cap
+        ctx.save_for_backward(q, k, v, spans, slopes, o, lse)
+        if q.numel() == 0 or k.numel() == 0:
+            return o.zero_()
+        spans, batch = _spans_arg(spans, Sq)
+        slopes = None if slopes is None else slopes.contiguous()
+        with _on(q.device):
+            at = [_strides(t) for t in (q, k, v)]
+            check(native.lib().rb_span_f32_fwd(D, ptr(q), ptr(k), ptr(v), *map(addressof, at), ptr(spans), batch, ptr(slopes), ptr(o), ptr(lse), B, H, Hkv,
+                                               Sq, Sk, int(causal), scale, cap, stream_ptr()), "rb_span_f32_fwd")
+            count_launch()
+        return o
+
+    @staticmethod
+    def backward(ctx, dout):
+        if torch.is_grad_enabled():
+            raise RuntimeError("span attention has no second derivatives")
+        q, k, v, spans, slopes, o, lse = ctx.saved_tensors
+        causal, scale, cap = ctx.args
+        B, Sq, H, D = q.shape
+        Sk, Hkv = k.shape[1], k.shape[2]
+        dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+        none = (None,) * 5
+        if q.numel() == 0 or k.numel() == 0:
+            return dq.zero_(), dk.zero_(), dv.zero_(), *none
+        dout = _view(dout)
+        spans, batch = _spans_arg(spans, Sq)
+        slopes = None if slopes is None else slopes.contiguous()
+        with _on(q.device):
+            at = [_strides(t) for t in (q, k, v, dout)]
+            check(native.lib().rb_span_f32_bwd(D, ptr(q), ptr(k), ptr(v), *map(addressof, at[:3]), ptr(spans), batch, ptr(slopes), ptr(o), ptr(lse), ptr(dout),
+                                               addressof(at[3]), ptr(dq), ptr(dk), ptr(dv), B, H, Hkv, Sq, Sk, int(causal), scale, cap, stream_ptr()),
+                  "rb_span_f32_bwd")
+            count_launch()
+        return dq, dk, dv, *none
+
+
+def _span_f32(q, k, v, *args):
+    """Heads of other sizes as the next size that the kernels have, with zeros behind: they add nothing to a product, and come off again."""
+    D = q.shape[3]
+    full = next(n for n in (16, 32, 64, 128) if n >= D)
+    if full != D:
+        q, k, v = (torch.nn.functional.pad(t, (0, full - D)) for t in (q, k, v))
+    return _SpanF32Fn.apply(q, k, v, *args)[..., :D]
+
+
 # ---------------------------------------------------------------- plain math
 def _weights(raw, distance, seen, slopes, cap: float):
     """Softmax weights of scaled products ``[..., heads, rows, keys]``; rows that see nothing get zeros."""
@@ -259,14 +317,18 @@ def span_attention(q, k, v, spans=None, causal: bool = True, scale: Optional[flo
     ``spans``: int32 ``[B, Sq, 2]`` (or ``[Sq, 2]`` for all batches), row i sees the keys ``lo <= j < hi``; parts outside the keys count as cut off, and
     a row with ``hi <= lo`` gives zeros.  ``causal``: besides, no key behind place ``i + Sk - Sq``.  ``cap``: scores s become cap tanh(s / cap), 0: they
     stay.  ``slopes``: float32 ``[H]``, what a score loses per place of distance (constants).  Keys and values have to be finite, unseen ones too: a
-    weight of zero times what is not finite is not a number.  On a GPU: bfloat16 or float16, D a multiple of 8 up to 128."""
+    weight of zero times what is not finite is not a number.  On a GPU: bfloat16 or float16 with D a multiple of 8 up to 128, float32 with D up to 128 (a kernel
+    for small models: rows are serial there)."""
     scale = float(scale) if scale is not None else 1.0 / math.sqrt(q.shape[-1])
     cap = float(cap)
     _rows_ok(q, k, v, spans, scale, cap, slopes)
     if not q.is_cuda:
         return span_reference(q, k, v, spans, causal, scale, cap, slopes)
+    if q.dtype == torch.float32 and q.shape[3] <= 128:
+        return _span_f32(q, k, v, spans, bool(causal), scale, cap, slopes)
     if not kernels_take(q):
-        raise TypeError(f"span attention on a GPU takes bfloat16 or float16 heads of a multiple of 8 numbers up to 128, not {q.dtype} of {q.shape[-1]}")
+        raise TypeError(f"span attention on a GPU takes bfloat16 or float16 heads of a multiple of 8 numbers up to 128, or float32 ones up to 128, not "
+                        f"{q.dtype} of {q.shape[-1]}")
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _SpanAttnFn.apply(q, k, v, spans, bool(causal), scale, cap, slopes)
     return span_forward(q, k, v, spans, bool(causal), scale, cap, slopes, lse=False)[0]

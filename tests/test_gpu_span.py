@@ -221,7 +221,7 @@ def test_parts_of_long_rows(Sq, Sk, H, cap):
 def test_refusals():
     from rumus_b200.ops import functional as F
     q, k, v, _ = _inputs(1, 16, 16, 4, 2, 64, BF)
-    for bad in (dict(q=q.float(), k=k.float(), v=v.float()), dict(q=q[..., :60], k=k[..., :60], v=v[..., :60]),
+    for bad in (dict(q=q.double(), k=k.double(), v=v.double()), dict(q=q[..., :60], k=k[..., :60], v=v[..., :60]),
                 dict(q=torch.cat([q, q, q], -1), k=torch.cat([k, k, k], -1), v=torch.cat([v, v, v], -1))):
         with pytest.raises(TypeError):
             F.span_attention(**bad)
