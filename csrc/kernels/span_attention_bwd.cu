@@ -25,7 +25,7 @@ struct SpanBwdParams {
   // per row, rows padded to a multiple of 64 (zeros there)
   float *row_lse2, *row_delta;      // [B, H, sq_pad], both negated
   int *row_lo, *row_hi;             // [B, sq_pad]
-  int4* range;                      // [B, sq_pad / 32] {least lo, largest hi, largest lo, least hi} of 32 rows
+  int4* range;                      // [B, sq_pad / 32], with a cap and a bias [B, H, sq_pad / 32]: span_range_warp of 32 rows
   int sq_pad;
   int* status;
 };
@@ -109,7 +109,7 @@ __global__ void __launch_bounds__(320, 1)
   int2 span = make_int2(0, 0);
   if (warp < 8) {
     if (live) span = span_of(p.c, b, row, p.Sq, p.Sk);
-    const int4 r = span_range_warp(span, live);
+    const int4 r = span_range_warp(span, CAP && BIAS ? span_near(span, row + off, span_reach(p.c, p.c.slopes[h])) : span, live);
     if (warp < 4 && lane == 0) s_range[warp] = r;
   } else if (warp == 9) {
     tmem_alloc(smem_u32(tmem_ptr), 512);
@@ -192,11 +192,11 @@ __global__ void __launch_bounds__(320, 1)
       if (h == 0) {
         p.row_lo[static_cast<long long>(b) * p.sq_pad + row] = span.x;
         p.row_hi[static_cast<long long>(b) * p.sq_pad + row] = span.y;
-        if (lane == 0) {
-          int4 r = s_range[warp];
-          if (row + 32 > p.Sq) r.w = 0;           // rows behind the last one see nothing: their scores are masked
-          p.range[(static_cast<long long>(b) * p.sq_pad + row) / 32] = r;
-        }
+      }
+      if (lane == 0 && (CAP && BIAS || h == 0)) {
+        int4 r = s_range[warp];
+        if (row + 32 > p.Sq) r.w = 0;             // rows behind the last one see nothing: their scores are masked
+        p.range[(static_cast<long long>(CAP && BIAS ? unit : b) * p.sq_pad + row) / 32] = r;
       }
     }
     // first guess of delta: dO.O, half of the columns each.  By way of shared memory: a thread's own row of loads, 16 bytes of a line each, took 10000 cycles.
@@ -373,14 +373,17 @@ __global__ void __launch_bounds__(320, 1)
   uint64_t *kv_full = bars, *full = bars + 1, *empty = full + C::STAGES, *st_full = empty + C::STAGES, *ready = st_full + 2, *all_done = ready + 2;
   uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(all_done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_ptr + 1);
-  __shared__ int s_first, s_last;
+  // with a cap and a bias each head reaches its own tiles; what many heads share a key head, those from the last slot on have their union
+  constexpr int SLOTS = CAP && BIAS ? 64 : 1;
+  __shared__ int s_first[SLOTS], s_last[SLOTS];
 
   const int warp = uniform_warp_idx(), lane = threadIdx.x & 31;
   int kv_tile, unit;
   span_place<false>(p.order, blockIdx.x, kv_tile, unit);      // causal: the keys that most rows see first
   const int kv0 = kv_tile * 128, hkv = unit % p.Hkv, b = unit / p.Hkv, group = p.H / p.Hkv;
   const int off = p.Sk - p.Sq, q_tiles = p.sq_pad / 64;
-  const int4* range = p.range + static_cast<long long>(b) * q_tiles * 2;
+  const int4* range = p.range + static_cast<long long>(CAP && BIAS ? b * p.H + hkv * group : b) * q_tiles * 2;
+  const int per_range = CAP && BIAS ? q_tiles * 2 : 0;          // from a head's to the next one's
 
   if (threadIdx.x == 0) {
     prefetch_tensormap(&tq);
@@ -398,8 +401,10 @@ __global__ void __launch_bounds__(320, 1)
     }
     mbar_init(smem_u32(all_done), 1);
     *abort_flag = 0;
-    s_first = 0x7fffffff;
-    s_last = -1;
+    for (int i = 0; i < SLOTS; ++i) {
+      s_first[i] = 0x7fffffff;
+      s_last[i] = -1;
+    }
     fence_barrier_init();
   }
   if (warp == 9) {
@@ -411,27 +416,38 @@ __global__ void __launch_bounds__(320, 1)
   tc_fence_after();
   const uint32_t tmem_base = *tmem_ptr;
   // query tiles from the first to the last that reaches these keys (what lies between and does not is masked)
-  for (int i = threadIdx.x; i < q_tiles; i += 320) {
+  const int lists = CAP && BIAS ? group : 1;
+  for (int i = threadIdx.x; i < q_tiles * lists; i += 320) {
+    const int g = i / q_tiles, tile = i - g * q_tiles;
     const int4 r = span_range_join(range[2 * i], range[2 * i + 1]);
     if (r.x < kv0 + 128 && r.y > kv0) {
-      atomicMin(&s_first, i);
-      atomicMax(&s_last, i);
+      atomicMin(&s_first[min(g, SLOTS - 1)], tile);
+      atomicMax(&s_last[min(g, SLOTS - 1)], tile);
     }
   }
   __syncthreads();
-  const int tile0 = s_first, per_head = s_last < 0 ? 0 : s_last + 1 - tile0;
-  const int n = per_head * group;
-  // the sweep's tiles in turn: query tiles of the first head, then of the next
+  // the sweep's tiles in turn: query tiles of the first head that has any, then of the next
   struct Place {
-    int h, tile;
+    int g, tile;
+  };
+  auto seek = [&](Place& c) {
+    while (c.g < group && s_last[min(c.g, SLOTS - 1)] < 0) ++c.g;
+    c.tile = c.g < group ? s_first[min(c.g, SLOTS - 1)] : 0;
   };
   auto next = [&](Place& c) {
-    if (++c.tile == tile0 + per_head) {
-      c.tile = tile0;
-      ++c.h;
+    if (++c.tile > s_last[min(c.g, SLOTS - 1)]) {
+      ++c.g;
+      seek(c);
     }
   };
-  const Place start = {hkv * group, tile0};
+  int n = 0;
+  if (SLOTS > 1) {
+    for (int g = 0; g < group; ++g) n += max(0, s_last[min(g, SLOTS - 1)] + 1 - s_first[min(g, SLOTS - 1)]);
+  } else if (s_last[0] >= 0) {
+    n = (s_last[0] + 1 - s_first[0]) * group;
+  }
+  Place start = {0, 0};
+  if (n > 0) seek(start);
 
   if (warp == 8) {
     // ------------------------------ TMA producer ------------------------------
@@ -449,7 +465,7 @@ __global__ void __launch_bounds__(320, 1)
       for (int it = 0; it < n; ++it, next(at)) {
         ok = mbar_wait(smem_u32(&empty[st]), ph ^ 1, abort_flag, p.status, RB_ERR_TIMEOUT_EMPTY);
         if (!ok) break;
-        const int h = at.h, tile = at.tile;
+        const int h = hkv * group + at.g, tile = at.tile;
         const uint32_t bar = smem_u32(&full[st]), dst = smem_u32(sQ + st * 2 * C::Q_TILE), rows = smem_u32(sRow + st * 1024);
         mbar_arrive_expect_tx(bar, 2 * C::Q_TILE + 1024);
         const long long bh = (static_cast<long long>(b) * p.H + h) * p.sq_pad + tile * 64, bb = static_cast<long long>(b) * p.sq_pad + tile * 64;
@@ -521,8 +537,8 @@ __global__ void __launch_bounds__(320, 1)
     int4 here = make_int4(0, 0, 0, 0);            // of the tile: asked for one tile ahead
     float slope_here = 0.f;
     auto ask = [&]() {
-      here = range[2 * at.tile + half];
-      if (BIAS) slope_here = __ldg(p.c.slopes + at.h);
+      here = range[at.g * per_range + 2 * at.tile + half];
+      if (BIAS) slope_here = __ldg(p.c.slopes + hkv * group + at.g);
     };
     if (n > 0) ask();
     for (int it = 0; it < n; ++it) {
@@ -708,8 +724,8 @@ int span_bwd(int dtype, const SpanBwdArrays& a, const SpanBwdParams& p, bool cap
 extern "C" {
 
 // Gradients of rb_span_fwd.  q, k, v, dout: 16-bit views as there; o contiguous and lse2 from the forward call with the same arguments.  dq [B, Sq, H, D]; dk and
-// dv [B, Sk, Hkv, D] of the same strides: views of 16-byte aligned rows.  scratch: 16-byte aligned, B pad (8 H + 8) + B pad / 2 bytes with pad = Sq rounded up to
-// a multiple of 64; nothing in it has to be set.
+// dv [B, Sk, Hkv, D] of the same strides: views of 16-byte aligned rows.  scratch: 16-byte aligned, B pad (8 H + 8) bytes and another B pad / 2, with a cap and
+// slopes B H pad / 2, with pad = Sq rounded up to a multiple of 64; nothing in it has to be set.
 int rb_span_bwd(int dtype, const void* q, const void* k, const void* v, const long long* qs, const long long* ks, const long long* vs, const int* spans,
                 long long span_batch, const float* slopes, const void* o, const float* lse2, const void* dout, const long long* dos, void* scratch, void* dq,
                 void* dk, void* dv, const long long* dqs, const long long* dkvs, int B, int H, int Hkv, int Sq, int Sk, int D, int causal, float scale,
@@ -717,6 +733,7 @@ int rb_span_bwd(int dtype, const void* q, const void* k, const void* v, const lo
   using namespace rb;
   if (B <= 0 || H <= 0 || Sq <= 0) return 0;
   if (Sk <= 0 || Hkv <= 0 || H % Hkv || D <= 0 || D > 128 || D % 8 || Sq > 0x7fffffff - 128) return 20;
+  if ((Sq + 63) / 64 * (static_cast<long long>(H) / Hkv) > 0x3fffffff) return 20;              // ranges of a key head's rows
   SpanBwdParams p{};
   p.B = B; p.H = H; p.Hkv = Hkv; p.Sq = Sq; p.Sk = Sk; p.D = D;
   p.c = rbh::span_scores(scale, cap);

@@ -88,7 +88,7 @@ __global__ void __launch_bounds__(SpanFwdCfg<HD>::THREADS, 1)
     const int row = q0 + threadIdx.x;
     const bool live = row < p.Sq;
     if (live) span = span_of(p.c, b, row, p.Sq, p.Sk);
-    const int4 r = span_range_warp(span, live);
+    const int4 r = span_range_warp(span, CAP && BIAS ? span_near(span, row + off, span_reach(p.c, p.c.slopes[h])) : span, live);
     if (lane == 0) s_range[warp] = r;
   } else if (warp == 9) {
     tmem_alloc(smem_u32(tmem_ptr), 512);

@@ -95,13 +95,21 @@ __global__ void __launch_bounds__(kSdWarps * 32, 2) span_decode_kernel(const Spa
   const int ctx = p.ctx[b];
   int end = static_cast<int>(min(static_cast<long long>(max(ctx, 0)), room));
   int begin = p.starts != nullptr ? max(p.starts[b], 0) : 0;
+  const int* table = p.tables + static_cast<long long>(b) * p.max_blocks;
+  if constexpr (CAP && BIAS) {
+    // what none of these heads gives a weight to is not read, provided that the nearest token is there
+    const int reach = __reduce_max_sync(0xffffffffu, lane < nh ? span_reach(p.c, p.c.slopes[h0 + lane]) : 0);
+    if (end - begin > reach) {
+      const int page = table[(end - 1) / p.page];
+      if (page >= 0 && page < p.pages) begin = end - 1 - reach;
+    }
+  }
   {
     const int n = max(0, end - begin), per = (n + p.splits * 64 - 1) / (p.splits * 64) * 64;      // whole trips of the CTA
     const long long from = begin + static_cast<long long>(sp) * per;
     begin = static_cast<int>(min(from, static_cast<long long>(end)));
     end = static_cast<int>(min(static_cast<long long>(end), from + per));
   }
-  const int* table = p.tables + static_cast<long long>(b) * p.max_blocks;
   const T *kc = reinterpret_cast<const T*>(p.k), *vc = reinterpret_cast<const T*>(p.v);
   const uint32_t ring = smem_u32(ring_all) + warp * kSdStages * C::STAGE;
 

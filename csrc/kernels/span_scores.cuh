@@ -11,6 +11,7 @@ struct SpanScores {
   float scale2;        // scale log2 e
   float in, out2;      // scale / cap, cap log2 e (cap)
   float near;          // products up to this size are near enough to zero for the tanh's polynomial (below zero: none is)
+  float far2;          // see span_reach; without a cap unused
   float k[4];          // its coefficients in the square of a product: tanh(in s) = s (k0 + k1 s^2 + k2 s^4 + k3 s^6)
   const float* slopes; // [H] or null
   const int2* spans;   // [B, Sq] {lo, hi} or null
@@ -29,6 +30,21 @@ __device__ __forceinline__ int2 span_of(const SpanScores& c, int b, int row, int
   }
   if (c.causal) s.y = min(s.y, row + Sk - Sq + 1);
   return s.x < s.y ? s : make_int2(0, 0);
+}
+
+// With a cap and a bias: how many places farther than a row's nearest key a key can be and still have a weight.  The nearest scores -cap - slope d or
+// more, one that is r places farther cap - slope (d + r) at most: from slope r = 2 cap + 150 log 2 on its weight is below 2^-150 of the nearest's, which is zero
+// in 32 bits whatever the products are.  Tiles that lie wholly there are left out.
+constexpr int kSpanNoReach = 0x7fffffff;
+__device__ __forceinline__ int span_reach(const SpanScores& c, float slope) {
+  const float r = c.far2 / (slope * kLog2e);
+  return slope > 0.f && r < 2e9f ? static_cast<int>(r) + 2 : kSpanNoReach;
+}
+// The part of a row's span that lies within `reach` of the key nearest to the row's place
+__device__ __forceinline__ int2 span_near(int2 s, int place, int reach) {
+  if (s.x >= s.y) return s;
+  const long long w = static_cast<long long>(max(0, max(s.x - place, place - (s.y - 1)))) + reach;
+  return make_int2(static_cast<int>(max(static_cast<long long>(s.x), place - w)), static_cast<int>(min(static_cast<long long>(s.y), place + w + 1)));
 }
 
 __device__ __forceinline__ uint64_t pair_at(const uint32_t* s, int i) { return f32x2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])); }
@@ -155,13 +171,13 @@ __device__ __forceinline__ void span_place(const SpanOrder& o, int idx, int& til
   unit = g * o.group + in - t * n;
 }
 
-// Range of keys that rows of a tile reach, over the `live` lanes of a warp: {least lo, largest hi, largest lo, least hi}; a row without keys keeps
-// the tile from being whole.
-__device__ __forceinline__ int4 span_range_warp(int2 s, bool live) {
-  const bool sees = live && s.x < s.y;
+// Range of keys that rows of a tile reach, over the `live` lanes of a warp: {least lo, largest hi of what is `near`, largest lo, least hi of the spans}; a
+// row without keys keeps the tile from being whole.
+__device__ __forceinline__ int4 span_range_warp(int2 s, int2 near, bool live) {
+  const bool sees = live && near.x < near.y;
   int4 r;
-  r.x = __reduce_min_sync(0xffffffffu, sees ? s.x : 0x7fffffff);
-  r.y = __reduce_max_sync(0xffffffffu, sees ? s.y : 0);
+  r.x = __reduce_min_sync(0xffffffffu, sees ? near.x : 0x7fffffff);
+  r.y = __reduce_max_sync(0xffffffffu, sees ? near.y : 0);
   r.z = __reduce_max_sync(0xffffffffu, live ? s.x : 0);
   r.w = __reduce_min_sync(0xffffffffu, live ? s.y : 0x7fffffff);
   return r;
@@ -184,6 +200,7 @@ inline rb::SpanScores span_scores(float scale, float cap) {
   if (!(cap > 0.f)) return c;
   c.in = scale / cap;
   c.out2 = cap * rb::kLog2e;
+  c.far2 = 2.f * c.out2 + 150.f;
   const float a = c.in < 0.f ? -c.in : c.in, w = c.in * c.in;
   const int terms = a > 0x1p-17f ? 4 : a > 0x1p-24f ? 3 : a > 0x1p-41f ? 2 : 1;
   c.near = (terms == 4 ? 0.625f : terms == 3 ? 0.2f : terms == 2 ? 0.07f : 0.003f) / a;

@@ -192,7 +192,8 @@ def span_backward(q, k, v, spans, causal: bool, scale: float, cap: float, slopes
         slopes = slopes.contiguous()
     with _on(q.device):
         rows = B * ((Sq + 63) // 64) * 64
-        scratch = torch.empty(rows * (8 * H + 8) + rows // 32 * 16, dtype=torch.uint8, device=q.device)
+        ranges = rows // 32 * 16 * (H if cap > 0 and slopes is not None else 1)
+        scratch = torch.empty(rows * (8 * H + 8) + ranges, dtype=torch.uint8, device=q.device)
         st = _strides(q), _strides(k), _strides(v), _strides(dout), _strides(dq), _strides(dk)
         at = [addressof(s) for s in st]
         check(native.lib().rb_span_bwd(native.dtype_code(q.dtype), ptr(q), ptr(k), ptr(v), at[0], at[1], at[2], ptr(spans), batch, ptr(slopes), ptr(o),

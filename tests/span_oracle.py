@@ -21,8 +21,11 @@ def seen_of(Sq, Sk, causal, spans, B, device):
 def span_oracle(q, k, v, spans=None, causal=True, scale=None, cap=0.0, slopes=None, dout=None):
     """{o, lse2, and with ``dout`` dq, dk, dv}, and per result the bound on the error of 16-bit kernels.  A rounding is off by half a step, u = eps / 2 of
     the value: results once; the weights (before P V and P^T dO) and dS (before dS K and dS^T Q) once more, so that what a sum is made of counts in
-    absolute values; delta = dO.O takes the rounded O."""
+    absolute values; delta = dO.O takes the rounded O.  fp16 has 10 bits behind the point down to 2^-14 and the same step, 2^-24, below: a weight or
+    dS smaller than that is off by up to half of it, 2^-25, whatever its size (weights relative to the row's largest score or to the sum, where none
+    counts more than that)."""
     u = torch.finfo(q.dtype).eps / 2
+    low = 2.0 ** -25 if q.dtype == torch.float16 else 0.0
     B, Sq, H, D = q.shape
     Sk, Hkv = k.shape[1], k.shape[2]
     G = H // Hkv
@@ -38,12 +41,13 @@ def span_oracle(q, k, v, spans=None, causal=True, scale=None, cap=0.0, slopes=No
         i, j = torch.arange(Sq, device=q.device)[:, None] + Sk - Sq, torch.arange(Sk, device=q.device)
         x = x - slopes.double().view(-1, 1, 1) * (i - j).abs()
     seen = seen_of(Sq, Sk, causal, spans, B, q.device)[:, None]
+    step = low * seen.double()
     x = x.masked_fill(~seen, -math.inf)
     p = torch.softmax(x, -1).nan_to_num(0.0)
     slip = slip * seen
     o = p @ vd
     r = {"o": o, "lse2": torch.logsumexp(x, -1) / math.log(2)}
-    e = {"o": u * o.abs() + (u + SLACK) * (p @ vd.abs())}
+    e = {"o": u * o.abs() + ((u + SLACK) * p + step) @ vd.abs()}
     if dout is not None:
         g = dout.double().transpose(1, 2)
         dp = g @ vd.transpose(-1, -2)
@@ -51,10 +55,10 @@ def span_oracle(q, k, v, spans=None, causal=True, scale=None, cap=0.0, slopes=No
         ds = p * (dp - delta) * slip
         # sizes of what is rounded, and of what rounding O does to delta
         off = (u + SLACK) * ds.abs() + SLACK * p * ((g.abs() @ vd.abs().transpose(-1, -2)) + (g.abs() * o.abs()).sum(-1, keepdim=True)) \
-            + p * slip * (g.abs() * e["o"]).sum(-1, keepdim=True)
+            + p * slip * (g.abs() * e["o"]).sum(-1, keepdim=True) + step
         r["dq"], e_dq = scale * (ds @ kd), abs(scale) * (off @ kd.abs())
         dk, e_dk = scale * (ds.transpose(-1, -2) @ qd), abs(scale) * (off.transpose(-1, -2) @ qd.abs())
-        dv, e_dv = p.transpose(-1, -2) @ g, (u + SLACK) * (p.transpose(-1, -2) @ g.abs())
+        dv, e_dv = p.transpose(-1, -2) @ g, ((u + SLACK) * p + step).transpose(-1, -2) @ g.abs()
         r["dk"], r["dv"], e_dk, e_dv = (t.view(B, Hkv, G, Sk, D).sum(2) for t in (dk, dv, e_dk, e_dv))
         e["dq"], e["dk"], e["dv"] = e_dq + u * r["dq"].abs(), e_dk + u * r["dk"].abs(), e_dv + u * r["dv"].abs()
     tiny = torch.finfo(q.dtype).tiny * torch.finfo(q.dtype).eps if q.dtype == torch.float16 else 0.0     # fp16 results below its normal numbers
