@@ -27,6 +27,10 @@ struct SpanBwdParams {
   int *row_lo, *row_hi;             // [B, sq_pad]
   int4* range;                      // [B, sq_pad / 32], with a cap and a bias [B, H, sq_pad / 32]: span_range_warp of 32 rows
   int sq_pad;
+  void *dk, *dv;                    // [B, Sk, Hkv, D], dkvs: strides {batch, row, head}
+  long long dkvs[3];
+  int parts;                        // CTAs that share a tile of keys
+  float* sums;                      // several parts: [parts, B, Hkv, tiles of 128 keys][dV, dK][HD / 32][128 keys][32, 16-byte pieces swizzled by the key]
   int* status;
 };
 
@@ -214,6 +218,7 @@ __global__ void __launch_bounds__(320, 1)
         guess = fmaf(e.x, f.x, fmaf(e.y, f.y, guess));
       }
     }
+    fence_proxy_async_smem();                                // what was read before what a copy writes in its place: without it loads are still under way
     mbar_arrive(smem_u32(rows_read));
     s_sum[0][wg][t] = guess;
     asm volatile("bar.sync 1, 256;" ::: "memory");          // the softmax warps, also where a wait ran out
@@ -357,6 +362,10 @@ struct SpanDkvCfg {
   static constexpr int ST_COL = 0, DP_COL = 128, DV_COL = 256, DK_COL = 384;     // S^T, dP^T of buffer w: + 64 w
 };
 
+__device__ __forceinline__ void bulk_store_1d(float* dst, uint32_t src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(src), "r"(bytes) : "memory");
+}
+
 template <typename T, int HD, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(320, 1)
     span_dkv_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
@@ -379,7 +388,8 @@ __global__ void __launch_bounds__(320, 1)
 
   const int warp = uniform_warp_idx(), lane = threadIdx.x & 31;
   int kv_tile, unit;
-  span_place<false>(p.order, blockIdx.x, kv_tile, unit);      // causal: the keys that most rows see first
+  const int parts = p.parts, rank = blockIdx.x % parts;
+  span_place<false>(p.order, blockIdx.x / parts, kv_tile, unit);      // causal: the keys that most rows see first
   const int kv0 = kv_tile * 128, hkv = unit % p.Hkv, b = unit / p.Hkv, group = p.H / p.Hkv;
   const int off = p.Sk - p.Sq, q_tiles = p.sq_pad / 64;
   const int4* range = p.range + static_cast<long long>(CAP && BIAS ? b * p.H + hkv * group : b) * q_tiles * 2;
@@ -434,12 +444,15 @@ __global__ void __launch_bounds__(320, 1)
     while (c.g < group && s_last[min(c.g, SLOTS - 1)] < 0) ++c.g;
     c.tile = c.g < group ? s_first[min(c.g, SLOTS - 1)] : 0;
   };
-  auto next = [&](Place& c) {
-    if (++c.tile > s_last[min(c.g, SLOTS - 1)]) {
-      ++c.g;
-      seek(c);
+  auto skip = [&](Place& c, int tiles) {
+    for (int i = 0; i < tiles && c.g < group; ++i) {
+      if (++c.tile > s_last[min(c.g, SLOTS - 1)]) {
+        ++c.g;
+        seek(c);
+      }
     }
   };
+  auto next = [&](Place& c) { skip(c, parts); };
   int n = 0;
   if (SLOTS > 1) {
     for (int g = 0; g < group; ++g) n += max(0, s_last[min(g, SLOTS - 1)] + 1 - s_first[min(g, SLOTS - 1)]);
@@ -447,7 +460,11 @@ __global__ void __launch_bounds__(320, 1)
     n = (s_last[0] + 1 - s_first[0]) * group;
   }
   Place start = {0, 0};
-  if (n > 0) seek(start);
+  if (n > 0) {
+    seek(start);
+    skip(start, rank);
+  }
+  n = (n - rank + parts - 1) / parts;             // of this CTA: every parts-th one
 
   if (warp == 8) {
     // ------------------------------ TMA producer ------------------------------
@@ -618,7 +635,23 @@ __global__ void __launch_bounds__(320, 1)
       ok = __all_sync(0xffffffffu, ok);
       tc_fence_after();
     }
-    if (ok) {
+    if (parts > 1) {
+      // warps 0-3 take dV, warps 4-7 dK: sums of this part, in chunks [128 keys x 32 columns] that take the place of all that was there
+#pragma unroll 1
+      for (int c = 0; c < HD / 32; ++c) {
+        uint32_t r[32];
+        if (n > 0) {
+          tmem_ld_32x32b_x32(lane_addr + (half == 0 ? C::DV_COL : C::DK_COL) + c * 32, r);
+          tmem_ld_wait();
+        } else {
+#pragma unroll
+          for (int k = 0; k < 32; ++k) r[k] = 0;
+        }
+        uint8_t* to = smem + (half * (HD / 32) + c) * 16384 + t * 128;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) *reinterpret_cast<uint4*>(to + ((k ^ (t & 7)) << 4)) = make_uint4(r[4 * k], r[4 * k + 1], r[4 * k + 2], r[4 * k + 3]);
+      }
+    } else if (ok) {
       // warps 0-3 take dV, warps 4-7 dK: through shared memory, in the place of V and K, from there in whole rows
       uint8_t* stage = (half == 0 ? sV : sK) + t * 128;
       const float f = half == 0 ? 1.f : p.grad_scale;
@@ -644,7 +677,13 @@ __global__ void __launch_bounds__(320, 1)
     }
     fence_proxy_async_smem();
     asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory");          // these four warps, also where a wait ran out
-    if (t == 0 && ok) {
+    if (t == 0 && ok && parts > 1) {
+      float* to = p.sums + (((static_cast<long long>(rank) * p.order.units + unit) * p.order.tiles + kv_tile) * 2 + half) * (HD * 128);
+#pragma unroll
+      for (int c = 0; c < HD / 32; ++c) bulk_store_1d(to + c * 4096, smem_u32(smem) + (half * (HD / 32) + c) * 16384, 16384);
+      tma_store_commit();
+      tma_store_wait_read<0>();
+    } else if (t == 0 && ok) {
 #pragma unroll
       for (int s = 0; s < C::SUB; ++s)
         if (s * 64 < p.D) tma_store_4d(half == 0 ? &tdv : &tdk, smem_u32((half == 0 ? sV : sK) + s * C::KV_SUB), s * 64, kv0, hkv, b);
@@ -659,6 +698,28 @@ __global__ void __launch_bounds__(320, 1)
     tc_fence_after();
     tmem_dealloc(tmem_base, 512);
   }
+}
+
+// Adds up the parts of dK and dV, in their order: eight numbers a thread
+template <typename T, int HD>
+__global__ void __launch_bounds__(256) span_dkv_join_kernel(const SpanBwdParams p) {
+  const long long tiles = static_cast<long long>(p.order.tiles) * p.order.units, i = blockIdx.x * 256ll + threadIdx.x;
+  const int piece = i & 3, key = i >> 2 & 127, c = (i >> 9) % (HD / 16);
+  const long long tile = i / (32 * HD);
+  if (tile >= tiles) return;
+  const int unit = static_cast<int>(tile / p.order.tiles), kv = static_cast<int>(tile % p.order.tiles) * 128 + key, d = (c & (HD / 32 - 1)) * 32 + piece * 8;
+  if (kv >= p.Sk || d >= p.D) return;
+  const float* at = p.sums + (tile * (HD / 16) + c) * 4096 + key * 32;
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
+  for (int r = 0; r < p.parts; ++r, at += tiles * (HD * 256)) {
+    const float4 g = *reinterpret_cast<const float4*>(at + (((2 * piece) ^ (key & 7)) << 2)), e = *reinterpret_cast<const float4*>(at + (((2 * piece + 1) ^ (key & 7)) << 2));
+    x.x += g.x; x.y += g.y; x.z += g.z; x.w += g.w;
+    y.x += e.x; y.y += e.y; y.z += e.z; y.w += e.w;
+  }
+  const bool is_dk = c >= HD / 32;
+  const float f = is_dk ? p.grad_scale : 1.f;
+  T* to = reinterpret_cast<T*>(is_dk ? p.dk : p.dv) + unit / p.Hkv * p.dkvs[0] + kv * p.dkvs[1] + unit % p.Hkv * p.dkvs[2] + d;
+  *reinterpret_cast<uint4*>(to) = make_uint4(pack2<T>(x.x * f, x.y * f), pack2<T>(x.z * f, x.w * f), pack2<T>(y.x * f, y.y * f), pack2<T>(y.z * f, y.w * f));
 }
 
 struct SpanBwdArrays {
@@ -678,11 +739,12 @@ int launch_span_bwd(const SpanBwdMaps& m, SpanBwdParams p, cudaStream_t st) {
   if (e == cudaSuccess) e = cudaFuncSetAttribute(dkv, cudaFuncAttributeMaxDynamicSharedMemorySize, SpanDkvCfg<HD>::SMEM_BYTES);
   if (e != cudaSuccess) return 2000 + (int)e;
   const long long q_tiles = (p.Sq + 127) / 128, kv_tiles = (p.Sk + 127) / 128;
-  if (q_tiles * p.H * p.B > 0x7fffffffll || kv_tiles * p.Hkv * p.B > 0x7fffffffll) return 20;
+  if (q_tiles * p.H * p.B > 0x7fffffffll || kv_tiles * p.Hkv * p.B * (p.parts > HD / 8 ? p.parts : HD / 8) > 0x7fffffffll) return 20;
   p.order = {(int)q_tiles, p.H * p.B, rbh::span_group(static_cast<long long>(p.H) * p.B, 4ll * p.Sk * p.D * p.Hkv / p.H)};
   dq<<<(unsigned)(q_tiles * p.H * p.B), 320, SpanDqCfg<HD>::SMEM_BYTES, st>>>(m.q128, m.do128, m.o128, m.k64, m.v64, m.dq128, p);
   p.order = {(int)kv_tiles, p.Hkv * p.B, rbh::span_group(static_cast<long long>(p.Hkv) * p.B, 4ll * p.Sq * p.D * (p.H / p.Hkv))};
-  dkv<<<(unsigned)(kv_tiles * p.Hkv * p.B), 320, SpanDkvCfg<HD>::SMEM_BYTES, st>>>(m.q64, m.k128, m.v128, m.do64, m.dk128, m.dv128, p);
+  dkv<<<(unsigned)(kv_tiles * p.Hkv * p.B * p.parts), 320, SpanDkvCfg<HD>::SMEM_BYTES, st>>>(m.q64, m.k128, m.v128, m.do64, m.dk128, m.dv128, p);
+  if (p.parts > 1) span_dkv_join_kernel<T, HD><<<(unsigned)(kv_tiles * p.Hkv * p.B * (HD / 8)), 256, 0, st>>>(p);
   e = cudaGetLastError();
   return e == cudaSuccess ? 0 : 3000 + (int)e;
 }
@@ -723,16 +785,31 @@ int span_bwd(int dtype, const SpanBwdArrays& a, const SpanBwdParams& p, bool cap
 
 extern "C" {
 
+// CTAs that share a tile of 128 keys of a key head in rb_span_bwd, each with every parts-th tile of rows, 8 of them at least: as many as make two CTAs per SM,
+// twice that where heads `differ` in how far they reach (a cap and slopes).  Whole backward pass with 1 and with these parts, heads of 128: 4096 tokens, 8
+// heads over 1: 654 and 187 us (8 parts); 2048 tokens, 8 heads: 87.1 and 85.6 (2); 8192 tokens, 16 heads over 4, capped and biased: 940 and 750 (2), where
+// the CTAs of the last key head would be at work alone.  Further parts cost 128 KB of sums a CTA: 4 x 2048 tokens, 16 heads over 4, whose 256 CTAs differ by
+// their place only: 326 with 1 part, 360 with 2.
+int rb_span_bwd_parts(int B, int H, int Hkv, int Sq, int Sk, int differ) {
+  if (B <= 0 || Hkv <= 0 || H <= 0 || Sq <= 0 || Sk <= 0) return 1;
+  const long long tiles = static_cast<long long>(B) * Hkv * ((Sk + 127ll) / 128), each = static_cast<long long>(H) / Hkv * ((Sq + 63ll) / 64);
+  long long parts = (differ ? 4ll : 2ll) * rbh::sm_count() / tiles;
+  if (parts > each / 8) parts = each / 8;
+  return parts < 1 ? 1 : parts > 8 ? 8 : static_cast<int>(parts);
+}
+
 // Gradients of rb_span_fwd.  q, k, v, dout: 16-bit views as there; o contiguous and lse2 from the forward call with the same arguments.  dq [B, Sq, H, D]; dk and
 // dv [B, Sk, Hkv, D] of the same strides: views of 16-byte aligned rows.  scratch: 16-byte aligned, B pad (8 H + 8) bytes and another B pad / 2, with a cap and
-// slopes B H pad / 2, with pad = Sq rounded up to a multiple of 64; nothing in it has to be set.
+// slopes B H pad / 2, with pad = Sq rounded up to a multiple of 64; nothing in it has to be set.  sums: with
+// several parts fp32 [parts, B, Hkv, Sk rounded up to 128, 2, 64 or 128 (D)], 16-byte aligned.
 int rb_span_bwd(int dtype, const void* q, const void* k, const void* v, const long long* qs, const long long* ks, const long long* vs, const int* spans,
-                long long span_batch, const float* slopes, const void* o, const float* lse2, const void* dout, const long long* dos, void* scratch, void* dq,
-                void* dk, void* dv, const long long* dqs, const long long* dkvs, int B, int H, int Hkv, int Sq, int Sk, int D, int causal, float scale,
-                float cap, void* stream) {
+                long long span_batch, const float* slopes, const void* o, const float* lse2, const void* dout, const long long* dos, void* scratch, float* sums,
+                void* dq, void* dk, void* dv, const long long* dqs, const long long* dkvs, int B, int H, int Hkv, int Sq, int Sk, int D, int parts, int causal,
+                float scale, float cap, void* stream) {
   using namespace rb;
   if (B <= 0 || H <= 0 || Sq <= 0) return 0;
   if (Sk <= 0 || Hkv <= 0 || H % Hkv || D <= 0 || D > 128 || D % 8 || Sq > 0x7fffffff - 128) return 20;
+  if (parts < 1 || (parts > 1 && !sums)) return 20;
   if ((Sq + 63) / 64 * (static_cast<long long>(H) / Hkv) > 0x3fffffff) return 20;              // ranges of a key head's rows
   SpanBwdParams p{};
   p.B = B; p.H = H; p.Hkv = Hkv; p.Sq = Sq; p.Sk = Sk; p.D = D;
@@ -743,6 +820,8 @@ int rb_span_bwd(int dtype, const void* q, const void* k, const void* v, const lo
   p.c.causal = causal;
   p.grad_scale = cap > 0.f ? -scale : scale;
   p.lse2 = lse2;
+  p.parts = parts; p.sums = sums; p.dk = dk; p.dv = dv;
+  for (int i = 0; i < 3; ++i) p.dkvs[i] = dkvs[i];
   p.sq_pad = (Sq + 63) / 64 * 64;
   const long long rows = static_cast<long long>(B) * p.sq_pad;
   p.row_lse2 = reinterpret_cast<float*>(scratch);

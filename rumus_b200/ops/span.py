@@ -24,7 +24,8 @@ from ._lib import check, count_launch, ptr, stream_ptr
 P, LL, I, Fl = c_void_p, c_longlong, c_int, c_float
 native.register_signature("rb_span_fwd_splits", [I, I, I, I])
 native.register_signature("rb_span_fwd", [I] + [P] * 7 + [LL] + [P] * 5 + [I] * 8 + [Fl, Fl, P])
-native.register_signature("rb_span_bwd", [I] + [P] * 7 + [LL] + [P] * 11 + [I] * 7 + [Fl, Fl, P])
+native.register_signature("rb_span_bwd_parts", [I] * 6)
+native.register_signature("rb_span_bwd", [I] + [P] * 7 + [LL] + [P] * 12 + [I] * 8 + [Fl, Fl, P])
 native.register_signature("rb_span_f32_fwd", [I] + [P] * 7 + [LL] + [P] * 3 + [I] * 6 + [Fl, Fl, P])
 native.register_signature("rb_span_f32_bwd", [I] + [P] * 7 + [LL] + [P] * 8 + [I] * 6 + [Fl, Fl, P])
 native.register_signature("rb_span_decode_splits", [I, I, I, I])
@@ -192,14 +193,18 @@ def span_backward(q, k, v, spans, causal: bool, scale: float, cap: float, slopes
         slopes = slopes.contiguous()
     with _on(q.device):
         rows = B * ((Sq + 63) // 64) * 64
-        ranges = rows // 32 * 16 * (H if cap > 0 and slopes is not None else 1)
-        scratch = torch.empty(rows * (8 * H + 8) + ranges, dtype=torch.uint8, device=q.device)
+        differ = cap > 0 and slopes is not None            # heads reach differently far
+        scratch = torch.empty(rows * (8 * H + 8) + rows // 32 * 16 * (H if differ else 1), dtype=torch.uint8, device=q.device)
+        L, sums = native.lib(), None
+        parts = L.rb_span_bwd_parts(B, H, Hkv, Sq, Sk, int(differ))
+        if parts > 1:
+            sums = torch.empty((parts, B, Hkv, (Sk + 127) // 128 * 128, 2, 64 if D <= 64 else 128), dtype=torch.float32, device=q.device)
         st = _strides(q), _strides(k), _strides(v), _strides(dout), _strides(dq), _strides(dk)
         at = [addressof(s) for s in st]
-        check(native.lib().rb_span_bwd(native.dtype_code(q.dtype), ptr(q), ptr(k), ptr(v), at[0], at[1], at[2], ptr(spans), batch, ptr(slopes), ptr(o),
-                                       ptr(lse2), ptr(dout), at[3], ptr(scratch), ptr(dq), ptr(dk), ptr(dv), at[4], at[5], B, H, Hkv, Sq, Sk, D,
-                                       int(causal), scale, cap, stream_ptr()), "rb_span_bwd")
-        count_launch(2)
+        check(L.rb_span_bwd(native.dtype_code(q.dtype), ptr(q), ptr(k), ptr(v), at[0], at[1], at[2], ptr(spans), batch, ptr(slopes), ptr(o), ptr(lse2),
+                            ptr(dout), at[3], ptr(scratch), ptr(sums), ptr(dq), ptr(dk), ptr(dv), at[4], at[5], B, H, Hkv, Sq, Sk, D, parts, int(causal),
+                            scale, cap, stream_ptr()), "rb_span_bwd")
+        count_launch(3 if parts > 1 else 2)
     return dq, dk, dv
 
 

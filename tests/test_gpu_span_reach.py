@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from test_gpu_span import BF, HF, _check, _inputs, _random_spans, _slopes
+from test_gpu_span import BF, HF, _check, _inputs, _random_spans, _run, _slopes
 from test_gpu_span_decode import _case
 from test_gpu_span_decode import _check as _check_decode
 
@@ -43,6 +43,19 @@ def test_spans_in_any_order():
 def test_many_heads_share_a_key_head(group):
     q, k, v, do = _inputs(1, 400, 400, group, 1, 32, BF)
     _check(q, k, v, do, cap=2.0, slopes=_slopes(group, 16.0))
+
+
+# tiles of keys that one CTA, two, some and eight share; keys that few rows see leave some of them without any
+@pytest.mark.parametrize("B,S,H,Hkv,parts", [(8, 600, 8, 8, 1), (1, 700, 4, 2, 2), (2, 900, 8, 2, 7), (1, 1030, 8, 1, 8)])
+@pytest.mark.parametrize("D", [64, 80, 128])
+@pytest.mark.parametrize("spans", [False, True])
+def test_shared_tiles(B, S, H, Hkv, parts, D, spans):
+    from rumus_b200.ops import native
+    assert native.lib().rb_span_bwd_parts(B, H, Hkv, S, S, 0) == parts
+    q, k, v, do = _inputs(B, S, S, H, Hkv, D, BF)
+    got = _check(q, k, v, do, spans=_random_spans(B, S, S) if spans else None, cap=8.0)
+    again = _run(q, k, v, do, spans=_random_spans(B, S, S) if spans else None, cap=8.0)
+    assert all(torch.equal(got[n], again[n]) for n in got)
 
 
 @pytest.mark.parametrize("H,Hkv", [(4, 4), (8, 2), (40, 2)])
