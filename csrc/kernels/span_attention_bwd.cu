@@ -25,7 +25,7 @@ struct SpanBwdParams {
   // per row, rows padded to a multiple of 64 (zeros there)
   float *row_lse2, *row_delta;      // [B, H, sq_pad], both negated
   int *row_lo, *row_hi;             // [B, sq_pad]
-  int4* range;                      // [B, sq_pad / 32], with a cap and a bias [B, H, sq_pad / 32]: span_range_warp of 32 rows
+  int4* range;                      // [B, sq_pad / 32], with a bias [B, H, sq_pad / 32]: span_range_warp of 32 rows
   int sq_pad;
   void *dk, *dv;                    // [B, Sk, Hkv, D], dkvs: strides {batch, row, head}
   long long dkvs[3];
@@ -113,7 +113,7 @@ __global__ void __launch_bounds__(320, 1)
   int2 span = make_int2(0, 0);
   if (warp < 8) {
     if (live) span = span_of(p.c, b, row, p.Sq, p.Sk);
-    const int4 r = span_range_warp(span, CAP && BIAS ? span_near(span, row + off, span_reach(p.c, p.c.slopes[h])) : span, live);
+    const int4 r = span_range_warp(span, BIAS ? span_near(span, row + off, span_head_reach<CAP>(p.c, b, h, hkv, p.H, p.Hkv)) : span, live);
     if (warp < 4 && lane == 0) s_range[warp] = r;
   } else if (warp == 9) {
     tmem_alloc(smem_u32(tmem_ptr), 512);
@@ -197,10 +197,10 @@ __global__ void __launch_bounds__(320, 1)
         p.row_lo[static_cast<long long>(b) * p.sq_pad + row] = span.x;
         p.row_hi[static_cast<long long>(b) * p.sq_pad + row] = span.y;
       }
-      if (lane == 0 && (CAP && BIAS || h == 0)) {
+      if (lane == 0 && (BIAS || h == 0)) {
         int4 r = s_range[warp];
         if (row + 32 > p.Sq) r.w = 0;             // rows behind the last one see nothing: their scores are masked
-        p.range[(static_cast<long long>(CAP && BIAS ? unit : b) * p.sq_pad + row) / 32] = r;
+        p.range[(static_cast<long long>(BIAS ? unit : b) * p.sq_pad + row) / 32] = r;
       }
     }
     // first guess of delta: dO.O, half of the columns each.  By way of shared memory: a thread's own row of loads, 16 bytes of a line each, took 10000 cycles.
@@ -382,8 +382,8 @@ __global__ void __launch_bounds__(320, 1)
   uint64_t *kv_full = bars, *full = bars + 1, *empty = full + C::STAGES, *st_full = empty + C::STAGES, *ready = st_full + 2, *all_done = ready + 2;
   uint32_t* tmem_ptr = reinterpret_cast<uint32_t*>(all_done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_ptr + 1);
-  // with a cap and a bias each head reaches its own tiles; what many heads share a key head, those from the last slot on have their union
-  constexpr int SLOTS = CAP && BIAS ? 64 : 1;
+  // with a bias each head reaches its own tiles; what many heads share a key head, those from the last slot on have their union
+  constexpr int SLOTS = BIAS ? 64 : 1;
   __shared__ int s_first[SLOTS], s_last[SLOTS];
 
   const int warp = uniform_warp_idx(), lane = threadIdx.x & 31;
@@ -392,8 +392,8 @@ __global__ void __launch_bounds__(320, 1)
   span_place<false>(p.order, blockIdx.x / parts, kv_tile, unit);      // causal: the keys that most rows see first
   const int kv0 = kv_tile * 128, hkv = unit % p.Hkv, b = unit / p.Hkv, group = p.H / p.Hkv;
   const int off = p.Sk - p.Sq, q_tiles = p.sq_pad / 64;
-  const int4* range = p.range + static_cast<long long>(CAP && BIAS ? b * p.H + hkv * group : b) * q_tiles * 2;
-  const int per_range = CAP && BIAS ? q_tiles * 2 : 0;          // from a head's to the next one's
+  const int4* range = p.range + static_cast<long long>(BIAS ? b * p.H + hkv * group : b) * q_tiles * 2;
+  const int per_range = BIAS ? q_tiles * 2 : 0;          // from a head's to the next one's
 
   if (threadIdx.x == 0) {
     prefetch_tensormap(&tq);
@@ -426,7 +426,7 @@ __global__ void __launch_bounds__(320, 1)
   tc_fence_after();
   const uint32_t tmem_base = *tmem_ptr;
   // query tiles from the first to the last that reaches these keys (what lies between and does not is masked)
-  const int lists = CAP && BIAS ? group : 1;
+  const int lists = BIAS ? group : 1;
   for (int i = threadIdx.x; i < q_tiles * lists; i += 320) {
     const int g = i / q_tiles, tile = i - g * q_tiles;
     const int4 r = span_range_join(range[2 * i], range[2 * i + 1]);
@@ -786,7 +786,7 @@ int span_bwd(int dtype, const SpanBwdArrays& a, const SpanBwdParams& p, bool cap
 extern "C" {
 
 // CTAs that share a tile of 128 keys of a key head in rb_span_bwd, each with every parts-th tile of rows, 8 of them at least: as many as make two CTAs per SM,
-// twice that where heads `differ` in how far they reach (a cap and slopes).  Whole backward pass with 1 and with these parts, heads of 128: 4096 tokens, 8
+// twice that where heads `differ` in how far they reach (slopes and a cap or norms).  Whole backward pass with 1 and with these parts, heads of 128: 4096 tokens, 8
 // heads over 1: 654 and 187 us (8 parts); 2048 tokens, 8 heads: 87.1 and 85.6 (2); 8192 tokens, 16 heads over 4, capped and biased: 940 and 750 (2), where
 // the CTAs of the last key head would be at work alone.  Further parts cost 128 KB of sums a CTA: 4 x 2048 tokens, 16 heads over 4, whose 256 CTAs differ by
 // their place only: 326 with 1 part, 360 with 2.
@@ -798,12 +798,12 @@ int rb_span_bwd_parts(int B, int H, int Hkv, int Sq, int Sk, int differ) {
   return parts < 1 ? 1 : parts > 8 ? 8 : static_cast<int>(parts);
 }
 
-// Gradients of rb_span_fwd.  q, k, v, dout: 16-bit views as there; o contiguous and lse2 from the forward call with the same arguments.  dq [B, Sq, H, D]; dk and
-// dv [B, Sk, Hkv, D] of the same strides: views of 16-byte aligned rows.  scratch: 16-byte aligned, B pad (8 H + 8) bytes and another B pad / 2, with a cap and
-// slopes B H pad / 2, with pad = Sq rounded up to a multiple of 64; nothing in it has to be set.  sums: with
+// Gradients of rb_span_fwd.  q, k, v, dout: 16-bit views as there; o contiguous, lse2 and norms (or null) from the forward call with the same arguments.  dq [B, Sq, H, D]; dk and
+// dv [B, Sk, Hkv, D] of the same strides: views of 16-byte aligned rows.  scratch: 16-byte aligned, B pad (8 H + 8) bytes and another B pad / 2, with slopes
+// B H pad / 2, with pad = Sq rounded up to a multiple of 64; nothing in it has to be set.  sums: with
 // several parts fp32 [parts, B, Hkv, Sk rounded up to 128, 2, 64 or 128 (D)], 16-byte aligned.
 int rb_span_bwd(int dtype, const void* q, const void* k, const void* v, const long long* qs, const long long* ks, const long long* vs, const int* spans,
-                long long span_batch, const float* slopes, const void* o, const float* lse2, const void* dout, const long long* dos, void* scratch, float* sums,
+                long long span_batch, const float* slopes, const float* norms, const void* o, const float* lse2, const void* dout, const long long* dos, void* scratch, float* sums,
                 void* dq, void* dk, void* dv, const long long* dqs, const long long* dkvs, int B, int H, int Hkv, int Sq, int Sk, int D, int parts, int causal,
                 float scale, float cap, void* stream) {
   using namespace rb;
@@ -815,6 +815,7 @@ int rb_span_bwd(int dtype, const void* q, const void* k, const void* v, const lo
   p.B = B; p.H = H; p.Hkv = Hkv; p.Sq = Sq; p.Sk = Sk; p.D = D;
   p.c = rbh::span_scores(scale, cap);
   p.c.slopes = slopes;
+  p.c.norms = norms;
   p.c.spans = reinterpret_cast<const int2*>(spans);
   p.c.span_batch = span_batch;
   p.c.causal = causal;

@@ -88,7 +88,7 @@ __global__ void __launch_bounds__(SpanFwdCfg<HD>::THREADS, 1)
     const int row = q0 + threadIdx.x;
     const bool live = row < p.Sq;
     if (live) span = span_of(p.c, b, row, p.Sq, p.Sk);
-    const int4 r = span_range_warp(span, CAP && BIAS ? span_near(span, row + off, span_reach(p.c, p.c.slopes[h])) : span, live);
+    const int4 r = span_range_warp(span, BIAS ? span_near(span, row + off, span_head_reach<CAP>(p.c, b, h, hkv, p.H, p.Hkv)) : span, live);
     if (lane == 0) s_range[warp] = r;
   } else if (warp == 9) {
     tmem_alloc(smem_u32(tmem_ptr), 512);
@@ -489,6 +489,49 @@ __global__ void __launch_bounds__(SpanFwdCfg<HD>::THREADS, 1)
   }
 }
 
+// Largest squared length of each of 32 parts of a head's rows: heads of queries, then of keys (SpanScores::norms).  8 or 16 lanes a row, 16 bytes each.
+// Bound by reading both once: 84 MB (2 x 4096 rows, 32 heads and 8 of 128) in 17.7 us, 4.7 TB/s.
+template <typename T>
+__global__ void __launch_bounds__(256) span_norms_kernel(const T* q, const T* k, long long qb, long long qr, long long qh, long long kb, long long kr, long long kh,
+                                                         float* norms, int H, int Hkv, int Sq, int Sk, int D) {
+  __shared__ uint32_t most[8];
+  // neighbouring CTAs take neighbouring heads of the same rows
+  const int units = gridDim.x / 32, part = blockIdx.x / units, unit = blockIdx.x - part * units, head = unit % (H + Hkv), b = unit / (H + Hkv);
+  const bool of_q = head < H;
+  const int S = of_q ? Sq : Sk, per = (S + 31) / 32, begin = min(S, part * per), end = min(S, begin + per);
+  const long long step = of_q ? qr : kr;
+  const int lanes = D <= 64 ? 8 : 16, rows = 256 / lanes, d = (threadIdx.x % lanes) * 8;
+  const T* at = (of_q ? q + b * qb + head * qh : k + b * kb + (head - H) * kh) + d;
+  uint32_t mx = 0;
+  for (int r0 = begin; r0 < end; r0 += rows * 4) {
+    uint4 v[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int r = r0 + u * rows + threadIdx.x / lanes;
+      v[u] = r < end && d < D ? __ldg(reinterpret_cast<const uint4*>(at + r * step)) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const uint32_t w[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = unpack2<T>(w[i]);
+        sum = fmaf(f.x, f.x, fmaf(f.y, f.y, sum));
+      }
+      for (int o = lanes / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      mx = max(mx, __float_as_uint(sum));
+    }
+  }
+  mx = __reduce_max_sync(0xffffffffu, mx);
+  if ((threadIdx.x & 31) == 0) most[threadIdx.x >> 5] = mx;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 8; ++w) mx = max(mx, most[w]);
+    norms[static_cast<long long>(unit) * 32 + part] = __uint_as_float(mx);
+  }
+}
+
 template <typename T, int HD, bool CAP, bool BIAS>
 int launch_span_fwd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& to, const SpanFwdParams& p, unsigned grid,
                     cudaStream_t st) {
@@ -519,6 +562,14 @@ int span_fwd(int dtype, const void* q, const void* k, const void* v, const long 
   if (grid > 0x7fffffffll) return 20;
   p.order = {(p.Sq + 255) / 256, (int)units, rbh::span_group(units, 4ll * p.Sk * p.D * p.Hkv / (p.splits * p.H) + 1)};
   const bool bias = p.c.slopes != nullptr;
+  if (p.c.norms != nullptr) {
+    const long long n = static_cast<long long>(p.B) * (p.H + p.Hkv) * 32;
+    if (n > 0x7fffffffll) return 20;
+    span_norms_kernel<T><<<(unsigned)n, 256, 0, st>>>((const T*)q, (const T*)k, qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], const_cast<float*>(p.c.norms), p.H,
+                                                      p.Hkv, p.Sq, p.Sk, p.D);
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return 3000 + (int)e;
+  }
 #define RB_SPAN(HD_)                                                                                          \
   (cap ? bias ? launch_span_fwd<T, HD_, true, true>(tq, tk, tv, to, p, (unsigned)grid, st)                    \
               : launch_span_fwd<T, HD_, true, false>(tq, tk, tv, to, p, (unsigned)grid, st)                   \
@@ -545,9 +596,10 @@ int rb_span_fwd_splits(int B, int H, int Sq, int Sk) {
 
 // q [B, Sq, H, D], k and v [B, Sk, Hkv, D]: 16-bit views, strides {batch, row, head} in elements (multiples of 8), 16-byte aligned; D a multiple of 8, at
 // most 128.  o [B, Sq, H, D] contiguous, lse2 [B, H, Sq].  spans: rows {lo, hi} of int32, `span_batch` rows apart per batch, or null; slopes [H] or
-// null; cap 0: none.  splits > 1: part_o [splits, B, Sq, H, D] and part_lse2 [splits, B, H, Sq] are scratch.
+// null; cap 0: none.  splits > 1: part_o [splits, B, Sq, H, D] and part_lse2 [splits, B, H, Sq] are scratch.  norms: null, or
+// with slopes and no cap fp32 [B, H + Hkv, 32] to note lengths in, by which tiles too far for a weight are left out.
 int rb_span_fwd(int dtype, const void* q, const void* k, const void* v, const long long* qs, const long long* ks, const long long* vs, const int* spans,
-                long long span_batch, const float* slopes, void* o, float* lse2, float* part_o, float* part_lse2, int B, int H, int Hkv, int Sq, int Sk,
+                long long span_batch, const float* slopes, float* norms, void* o, float* lse2, float* part_o, float* part_lse2, int B, int H, int Hkv, int Sq, int Sk,
                 int D, int splits, int causal, float scale, float cap, void* stream) {
   using namespace rb;
   if (B <= 0 || H <= 0 || Sq <= 0) return 0;
@@ -557,6 +609,7 @@ int rb_span_fwd(int dtype, const void* q, const void* k, const void* v, const lo
   p.splits = splits;
   p.c = rbh::span_scores(scale, cap);
   p.c.slopes = slopes;
+  p.c.norms = slopes && !(cap > 0.f) ? norms : nullptr;
   p.c.spans = reinterpret_cast<const int2*>(spans);
   p.c.span_batch = span_batch;
   p.c.causal = causal;

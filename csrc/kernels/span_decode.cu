@@ -98,7 +98,7 @@ __global__ void __launch_bounds__(kSdWarps * 32, 2) span_decode_kernel(const Spa
   const int* table = p.tables + static_cast<long long>(b) * p.max_blocks;
   if constexpr (CAP && BIAS) {
     // what none of these heads gives a weight to is not read, provided that the nearest token is there
-    const int reach = __reduce_max_sync(0xffffffffu, lane < nh ? span_reach(p.c, p.c.slopes[h0 + lane]) : 0);
+    const int reach = __reduce_max_sync(0xffffffffu, lane < nh ? span_reach(p.c.far2, p.c.slopes[h0 + lane]) : 0);
     if (end - begin > reach) {
       const int page = table[(end - 1) / p.page];
       if (page >= 0 && page < p.pages) begin = end - 1 - reach;

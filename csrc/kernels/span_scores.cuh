@@ -11,7 +11,8 @@ struct SpanScores {
   float scale2;        // scale log2 e
   float in, out2;      // scale / cap, cap log2 e (cap)
   float near;          // products up to this size are near enough to zero for the tanh's polynomial (below zero: none is)
-  float far2;          // see span_reach; without a cap unused
+  float far2;          // see span_reach; without a cap 0
+  const float* norms;  // without a cap: [B, H + Hkv, 32] largest squared lengths of 32 parts of a head's queries, then of the key heads' keys; null: not known
   float k[4];          // its coefficients in the square of a product: tanh(in s) = s (k0 + k1 s^2 + k2 s^4 + k3 s^6)
   const float* slopes; // [H] or null
   const int2* spans;   // [B, Sq] {lo, hi} or null
@@ -32,13 +33,22 @@ __device__ __forceinline__ int2 span_of(const SpanScores& c, int b, int row, int
   return s.x < s.y ? s : make_int2(0, 0);
 }
 
-// With a cap and a bias: how many places farther than a row's nearest key a key can be and still have a weight.  The nearest scores -cap - slope d or
-// more, one that is r places farther cap - slope (d + r) at most: from slope r = 2 cap + 150 log 2 on its weight is below 2^-150 of the nearest's, which is zero
-// in 32 bits whatever the products are.  Tiles that lie wholly there are left out.
+// With a bias: how many places farther than a row's nearest key a key can be and still have a weight.  Where no score but for the bias is above m in size (the
+// cap, or |scale| times the largest query's and key's lengths) the nearest key has -m - slope d or more, one that is r places farther m - slope (d + r) at
+// most: from slope r = 2 m + 150 log 2 on its weight is below 2^-150 of the nearest's, which is zero in 32 bits.  Tiles that lie wholly there are left out.
 constexpr int kSpanNoReach = 0x7fffffff;
-__device__ __forceinline__ int span_reach(const SpanScores& c, float slope) {
-  const float r = c.far2 / (slope * kLog2e);
+__device__ __forceinline__ int span_reach(float far2, float slope) {          // far2: 2 m log2 e + 150
+  const float r = far2 / (slope * kLog2e);
   return slope > 0.f && r < 2e9f ? static_cast<int>(r) + 2 : kSpanNoReach;
+}
+// Of a head; whole warps.  The bits of lengths, which are not negative, are in the lengths' order, with what is no number above all.
+template <bool CAP>
+__device__ __forceinline__ int span_head_reach(const SpanScores& c, int b, int h, int hkv, int H, int Hkv) {
+  if (CAP) return span_reach(c.far2, c.slopes[h]);
+  if (c.norms == nullptr) return kSpanNoReach;
+  const float* of = c.norms + static_cast<long long>(b) * (H + Hkv) * 32 + (threadIdx.x & 31);
+  const uint32_t q2 = __reduce_max_sync(0xffffffffu, __float_as_uint(of[h * 32])), k2 = __reduce_max_sync(0xffffffffu, __float_as_uint(of[(H + hkv) * 32]));
+  return span_reach(2.002f * fabsf(c.scale2) * sqrtf(__uint_as_float(q2)) * sqrtf(__uint_as_float(k2)) + 150.f, c.slopes[h]);
 }
 // The part of a row's span that lies within `reach` of the key nearest to the row's place
 __device__ __forceinline__ int2 span_near(int2 s, int place, int reach) {

@@ -246,4 +246,4 @@ def test_launchers_refuse_what_they_cannot_do():
     L = native.lib()
     none = [None] * 3
     for D, H, Hkv, splits in ((136, 2, 2, 1), (12, 2, 2, 1), (64, 3, 2, 1), (64, 2, 2, 2)):
-        assert L.rb_span_fwd(2, *none, *none, None, 0, None, None, None, None, None, 1, H, Hkv, 4, 4, D, splits, 1, 1.0, 0.0, None) == 20
+        assert L.rb_span_fwd(2, *none, *none, None, 0, None, None, None, None, None, None, 1, H, Hkv, 4, 4, D, splits, 1, 1.0, 0.0, None) == 20

@@ -22,6 +22,19 @@ def test_far_tiles(B, Sq, Sk, causal, dtype):
     _check(q, k, v, do, causal=causal, cap=5.0, slopes=_steep(10.0, 1.0, 0.3, 0.0, -0.01, 1e-30))
 
 
+# without a cap the lengths of queries and keys say how far a score can be from zero: one of each is long here, and its scores win over the distance
+@pytest.mark.parametrize("B,Sq,Sk", [(1, 4200, 4200), (2, 1100, 4300)])
+@pytest.mark.parametrize("D,dtype", [(64, BF), (128, HF), (40, BF)])
+def test_far_tiles_without_a_cap(B, Sq, Sk, D, dtype):
+    from rumus_b200.ops import span
+    q, k, v, do = _inputs(B, Sq, Sk, 4, 2, D, dtype, spread=0.5)
+    q[:, Sq - 7, 1] *= 20
+    k[:, 5, 0] = q[:, Sq - 7, 1] / 4
+    slopes = _steep(2.0, 0.25, 0.05, -0.001)
+    assert span._norms(q, k, 0.0, slopes) is not None
+    _check(q, k, v, do, causal=Sq > 2000, slopes=slopes)
+
+
 # rows whose nearest key is far: the distance counts from there
 @pytest.mark.parametrize("causal", [True, False])
 def test_rows_whose_keys_are_all_far(causal):
