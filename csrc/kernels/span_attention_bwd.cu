@@ -438,18 +438,20 @@ __global__ void __launch_bounds__(320, 1)
   __syncthreads();
   // the sweep's tiles in turn: query tiles of the first head that has any, then of the next
   struct Place {
-    int g, tile;
+    int g, tile, last;
   };
   auto seek = [&](Place& c) {
     while (c.g < group && s_last[min(c.g, SLOTS - 1)] < 0) ++c.g;
     c.tile = c.g < group ? s_first[min(c.g, SLOTS - 1)] : 0;
+    c.last = c.g < group ? s_last[min(c.g, SLOTS - 1)] : 0x7fffffff;
   };
   auto skip = [&](Place& c, int tiles) {
-    for (int i = 0; i < tiles && c.g < group; ++i) {
-      if (++c.tile > s_last[min(c.g, SLOTS - 1)]) {
-        ++c.g;
-        seek(c);
-      }
+    c.tile += tiles;
+    while (c.tile > c.last) {
+      const int over = c.tile - c.last - 1;
+      ++c.g;
+      seek(c);
+      c.tile += over;
     }
   };
   auto next = [&](Place& c) { skip(c, parts); };
@@ -459,7 +461,7 @@ __global__ void __launch_bounds__(320, 1)
   } else if (s_last[0] >= 0) {
     n = (s_last[0] + 1 - s_first[0]) * group;
   }
-  Place start = {0, 0};
+  Place start = {0, 0, 0};
   if (n > 0) {
     seek(start);
     skip(start, rank);

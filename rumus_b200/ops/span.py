@@ -114,6 +114,10 @@ def _on(device):
     return _HERE if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
 
 
+def _like(t: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 _Strides = LL * 3
 
 
@@ -162,12 +166,12 @@ def span_forward(q, k, v, spans, causal: bool, scale: float, cap: float, slopes,
     B, Sq, H, D = q.shape
     Sk, Hkv = k.shape[1], k.shape[2]
     if out is None:
-        o = q.new_empty((B, Sq, H, D))
+        o = _like(q)
     elif not out.is_contiguous() or out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or out.data_ptr() % 16:
         raise ValueError(f"span attention writes contiguous heads {tuple(q.shape)} of {q.dtype}, not {out.dtype} {tuple(out.shape)}")
     else:
         o = out
-    lse2 = torch.empty((B, H, Sq), dtype=torch.float32, device=q.device) if lse else None
+    lse2 = q.new_empty((B, H, Sq), dtype=torch.float32) if lse else None
     if o.numel() == 0:
         return o, lse2
     if Sk == 0:
@@ -194,7 +198,7 @@ def span_backward(q, k, v, spans, causal: bool, scale: float, cap: float, slopes
     """dq, dk, dv.  ``norms``: those of the forward call.  ``out``: views of 16-byte aligned rows to write them into (dk and dv of the same strides)."""
     B, Sq, H, D = q.shape
     Sk, Hkv = k.shape[1], k.shape[2]
-    dq, dk, dv = out if out is not None else (q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape))
+    dq, dk, dv = out if out is not None else (_like(q), _like(k), _like(v))
     if q.numel() == 0 or k.numel() == 0:
         return dq.zero_(), dk.zero_(), dv.zero_()
     dout = _view(dout)
@@ -204,7 +208,7 @@ def span_backward(q, k, v, spans, causal: bool, scale: float, cap: float, slopes
     with _on(q.device):
         rows = B * ((Sq + 63) // 64) * 64
         differ = slopes is not None and (cap > 0 or norms is not None)            # heads reach differently far
-        scratch = torch.empty(rows * (8 * H + 8) + rows // 32 * 16 * (H if slopes is not None else 1), dtype=torch.uint8, device=q.device)
+        scratch = q.new_empty(rows * (8 * H + 8) + rows // 32 * 16 * (H if slopes is not None else 1), dtype=torch.uint8)
         L, sums = native.lib(), None
         parts = L.rb_span_bwd_parts(B, H, Hkv, Sq, Sk, int(differ))
         if parts > 1:
@@ -246,7 +250,7 @@ class _SpanF32Fn(torch.autograd.Function):
         q, k, v = _view(q), _view(k), _view(v)
         B, Sq, H, D = q.shape
         Sk, Hkv = k.shape[1], k.shape[2]
-        o, lse = q.new_empty(q.shape), q.new_empty((B, H, Sq))
+        o, lse = _like(q), q.new_empty((B, H, Sq))
         ctx.args = causal, scale, cap
         ctx.save_for_backward(q, k, v, spans, slopes, o, lse)
         if q.numel() == 0 or k.numel() == 0:
@@ -268,7 +272,7 @@ class _SpanF32Fn(torch.autograd.Function):
         causal, scale, cap = ctx.args
         B, Sq, H, D = q.shape
         Sk, Hkv = k.shape[1], k.shape[2]
-        dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+        dq, dk, dv = _like(q), _like(k), _like(v)
         none = (None,) * 5
         if q.numel() == 0 or k.numel() == 0:
             return dq.zero_(), dk.zero_(), dv.zero_(), *none
