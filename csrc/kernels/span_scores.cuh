@@ -223,10 +223,13 @@ inline rb::SpanScores span_scores(float scale, float cap) {
   return c;
 }
 
-// Heads whose streamed rows (`bytes` each) take a quarter of the L2 cache
+// Heads whose streamed rows (`bytes` each) take a quarter of the L2 cache, in groups of one size: with 63 heads and one more, whose longest tiles came last
+// of all, the SMs were idle for a sixth of a launch.
 inline int span_group(long long units, long long bytes) {
-  const long long fit = (32ll << 20) / (bytes > 0 ? bytes : 1);
-  return (int)(fit < 1 ? 1 : fit < units ? fit : units);
+  long long fit = (32ll << 20) / (bytes > 0 ? bytes : 1);
+  if (fit < 1) fit = 1;
+  const long long groups = (units + fit - 1) / fit;
+  return (int)(groups < 1 ? 1 : (units + groups - 1) / groups);
 }
 
 // Tensor map of heads [B, S, heads, D] with strides {batch, row, head} in elements, read in boxes of `rows` rows of 64 numbers of a head; what lies

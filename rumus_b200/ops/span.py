@@ -152,8 +152,8 @@ def _spans_arg(spans, rows: int):
 def _norms(q, k, cap: float, slopes):
     """Room for the lengths of queries and keys, by which biased scores without a cap are known to be too far for a weight; None where it does not pay.
     One pass over both is linear in the rows, what it saves grows with their square.  Without / with it, usual slopes: 2 x 4096 rows, 32 heads over 8 of 128:
-    forward 365 / 313 us, backward 1021 / 885; 8192 rows, 16 heads over 4: 272 / 188 and 980 / 634; 4 x 2048 rows, 16 heads of 64: 121 / 127 and 276 / 240;
-    512 rows over 8192 keys, 32 heads over 8: forward 181 / 192."""
+    forward 312 / 257 us, backward 993 / 844; 8192 rows, 16 heads over 4: 273 / 187 and 940 / 651; 4 x 2048 rows, 16 heads of 64: 100 / 105 and 281 / 247;
+    512 rows over 8192 keys, 32 heads over 8: forward 181 / 193."""
     if slopes is None or cap > 0 or q.shape[1] < 1024 or k.shape[1] < 4096:
         return None
     return torch.empty((q.shape[0], q.shape[2] + k.shape[2], 32), dtype=torch.float32, device=q.device)
