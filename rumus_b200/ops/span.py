@@ -142,10 +142,19 @@ def _strides(t: torch.Tensor):
 
 
 def _spans_arg(spans, rows: int):
-    """(contiguous spans, rows from one batch's to the next's)."""
+    """(contiguous spans, 8-byte aligned: the kernels read lo and hi at once; rows from one batch's to the next's)."""
     if spans is None:
         return None, 0
-    return spans.contiguous(), rows if spans.dim() == 3 else 0
+    spans = spans.contiguous()
+    return spans if spans.data_ptr() % 8 == 0 else spans.clone(), rows if spans.dim() == 3 else 0
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the memory that the views span has bytes in common."""
+    if a.numel() == 0 or b.numel() == 0 or a.device != b.device:
+        return False
+    (a0, a1), (b0, b1) = ((t.data_ptr(), t.data_ptr() + (sum((n - 1) * d for n, d in zip(t.shape, t.stride())) + 1) * t.element_size()) for t in (a, b))
+    return a0 < b1 and b0 < a1
 
 
 # ---------------------------------------------------------------- kernels
@@ -194,11 +203,11 @@ def span_forward(q, k, v, spans, causal: bool, scale: float, cap: float, slopes,
     return o, lse2
 
 
-def span_backward(q, k, v, spans, causal: bool, scale: float, cap: float, slopes, o, lse2, dout, out=None, norms=None):
-    """dq, dk, dv.  ``norms``: those of the forward call.  ``out``: views of 16-byte aligned rows to write them into (dk and dv of the same strides)."""
+def span_backward(q, k, v, spans, causal: bool, scale: float, cap: float, slopes, o, lse2, dout, norms=None):
+    """dq, dk, dv.  ``norms``: those of the forward call."""
     B, Sq, H, D = q.shape
     Sk, Hkv = k.shape[1], k.shape[2]
-    dq, dk, dv = out if out is not None else (_like(q), _like(k), _like(v))
+    dq, dk, dv = _like(q), _like(k), _like(v)
     if q.numel() == 0 or k.numel() == 0:
         return dq.zero_(), dk.zero_(), dv.zero_()
     dout = _view(dout)
@@ -363,7 +372,8 @@ def span_decode(q, k_cache, v_cache, block_tables, ctx_lens, max_ctx: int, scale
     Caches ``[pages, page, Hkv, D]``, with ``head_major`` ``[pages, Hkv, page, D]``; ``block_tables`` int32 ``[B, n]``; ``ctx_lens``, ``starts`` (None:
     0) int32 ``[B]``; ``max_ctx``: no context is longer (decides how contexts are cut; longer ones are still right).  Tokens in pages that the cache
     does not have, and behind the table's end, count as unseen; what pages hold behind a context is never read.  ``cap``, ``slopes``: as in
-    ``span_attention``.  ``out``: contiguous tensor to write into.  On a GPU: bfloat16 or float16, D a multiple of 8 up to 128."""
+    ``span_attention``.  ``out``: contiguous tensor to write into, apart from the others.  On a GPU: bfloat16 or float16, D a multiple of 8 up to
+    128."""
     if q.dim() != 3 or k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
         raise ValueError(f"decoding of {tuple(q.shape)} over pages {tuple(k_cache.shape)}, {tuple(v_cache.shape)}")
     B, H, D = q.shape
@@ -387,6 +397,8 @@ def span_decode(q, k_cache, v_cache, block_tables, ctx_lens, max_ctx: int, scale
         out = q.new_empty((B, H, D))
     elif not out.is_contiguous() or out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or out.data_ptr() % 8:
         raise ValueError(f"decoding writes contiguous heads {tuple(q.shape)} of {q.dtype}, not {out.dtype} {tuple(out.shape)}")
+    elif any(_overlap(out, t) for t in (q, k_cache, v_cache)):
+        raise ValueError("decoding reads its queries and pages while it writes: ``out`` has to be apart from them")
     if not q.is_cuda:
         return out.copy_(_decode_reference(q, k_cache, v_cache, block_tables, ctx_lens, scale, cap, slopes, starts, head_major))
     if not kernels_take(q):

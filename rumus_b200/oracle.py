@@ -132,6 +132,8 @@ class OracleDecoder:
     def __init__(self, cfg, batch: int):
         if getattr(cfg, "activation", "relu") != "relu":
             raise ValueError("the oracle decoder implements the ReLU feed-forward of the functional configuration")
+        if getattr(cfg, "attn_cap", 0.0) > 0 or getattr(cfg, "alibi", False):
+            raise ValueError("the oracle decoder has plain causal attention and a positional embedding")
         L = _L()
         L.orc_decoder_create.restype = c_void_p
         L.orc_decoder_tensor.restype = ctypes.POINTER(c_float)

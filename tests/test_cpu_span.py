@@ -1,4 +1,5 @@
 """Span attention's plain math, its spans and its refusals."""
+import dataclasses
 import math
 
 import pytest
@@ -138,5 +139,28 @@ def test_refusals():
                      ((q, k, v, tables, ctx, 8), dict(cap=-2.0))]:
         with pytest.raises(ValueError):
             span_decode(*args, **kw)
+    both = torch.randn(4, 2, 8, dtype=torch.float64)
+    span_decode(both[:1], k, v, tables, ctx, 8, out=both[1:2])
+    for out in (both[:1], k.view(-1)[:16].view(1, 2, 8)):
+        with pytest.raises(ValueError, match="apart"):
+            span_decode(both[:1], k, v, tables, ctx, 8, out=out)
     with pytest.raises(ValueError):
         distance_slopes(0)
+
+
+def test_spans_at_any_address_reach_the_kernels_aligned():
+    from rumus_b200.ops.span import _spans_arg
+    flat = torch.arange(2 * 5 * 2 + 3, dtype=torch.int32)
+    for first in range(3):
+        spans = flat[first:first + 20].view(2, 5, 2)
+        got, rows = _spans_arg(spans, 5)
+        assert got.data_ptr() % 8 == 0 and torch.equal(got, spans) and got.is_contiguous() and rows == 5
+    assert _spans_arg(flat[1:11].view(5, 2), 5)[1] == 0
+
+
+def test_the_oracle_decoder_refuses_shaped_scores():
+    from rumus_b200.models.gpt import GPTConfig
+    from rumus_b200.oracle import OracleDecoder
+    for kw in (dict(attn_cap=5.0), dict(alibi=True)):
+        with pytest.raises(ValueError, match="oracle"):
+            OracleDecoder(dataclasses.replace(GPTConfig.tiny_cpu(), **kw), 2)

@@ -86,3 +86,11 @@ def test_decode_without_the_last_page():
     tables[0, -1] = -1
     tables[1, 5:] = 10 ** 9
     _check_decode((q, k, v, tables, ctx), 4, cap=5.0, slopes=_steep(3.0, 2.0, 1.0, 0.5))
+
+
+def test_spans_at_an_odd_address():
+    q, k, v, do = _inputs(2, 90, 90, 2, 2, 64, BF)
+    spans = _random_spans(2, 90, 90)
+    odd = torch.cat([spans.view(-1)[:1], spans.view(-1)])[1:].view(2, 90, 2)
+    assert odd.data_ptr() % 8 == 4
+    _check(q, k, v, do, spans=odd)
