@@ -585,13 +585,16 @@ int span_fwd(int dtype, const void* q, const void* k, const void* v, const long 
 
 extern "C" {
 
-// Parts that the keys of a call are cut into: as many as fill the SMs once where the tiles of 256 rows alone leave half of them idle, each of four
-// tiles of 128 keys at least.
+// Parts that the keys of a call are cut into: as many as fill the SMs once where the tiles of 256 rows alone leave half of them idle, each of 256 keys at
+// least, 8 at most.  us at several numbers, heads of 128, the rule's in brackets: 512 rows over 8704 keys, 32 heads: 156 in 1 part, [93 in 2], 128 in 3; 1024
+// over 4096, 18 heads: 78.8 in 1, [57.9 in 2]; 20 heads: [78.7 in 1], 94.8 in 2; 256 over 1024, 32 heads: 26.1 in 1, [22.2 in 4], 35.7 in 6; 64 over 4096, 8
+// heads: 54.4 in 1, 22.2 in 4, [17.5 in 8], 19.5 in 16.
 int rb_span_fwd_splits(int B, int H, int Sq, int Sk) {
   const long long tiles = static_cast<long long>((Sq + 255) / 256) * B * H;
   if (tiles <= 0 || 2 * tiles > rbh::sm_count()) return 1;
-  const long long most = (static_cast<long long>(Sk) + 511) / 512, fill = rbh::sm_count() / tiles;
-  return static_cast<int>(most < 1 ? 1 : fill < most ? fill : most);
+  const long long most = (static_cast<long long>(Sk) + 255) / 256, fill = rbh::sm_count() / tiles;
+  const long long parts = fill < most ? fill : most;
+  return static_cast<int>(parts < 1 ? 1 : parts > 8 ? 8 : parts);
 }
 
 // q [B, Sq, H, D], k and v [B, Sk, Hkv, D]: 16-bit views, strides {batch, row, head} in elements (multiples of 8), 16-byte aligned; D a multiple of 8, at

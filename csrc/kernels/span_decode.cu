@@ -368,17 +368,21 @@ int span_decode(const SpanDecodeParams& p, bool cap, unsigned grid, cudaStream_t
 extern "C" {
 
 // Parts that contexts of up to max_ctx tokens are cut into, for B sequences of Hkv key heads that H query heads share: as many as fill every SM with two
-// CTAs, of 256 keys each at least.
+// CTAs, in a cluster of 2, 4 or 8 of one trip (64 keys) each at least, or, where 8 would have more than 1536 keys each, through memory, of 512 at least.  us at
+// several numbers, heads of 128, the rule's in brackets: 1 x 300 tokens, 32 heads over 8: 7.7 with 1 part, 7.0 with 2, [6.2 with 4], 5.6 with 8; 1 x 1100:
+// 17.8 with 1, 8.8 with 4, [7.4 with 8], 10.4 with 12; 8 x 32768: 204 with 2, [153 with 4], 158 with 8; 48 x 1250, 32 key heads: [158 with 1], 176 with 2;
+// over 2 heads of 64, 2 x 9000: [15.6 with 8], 17.3 with 18; 2 x 12000: [19.1 with 8], 18.3 with 24; 1 x 40000: 65.8 with 8, 34.8 with 24, [35.9 with 64].
 int rb_span_decode_splits(int B, int H, int Hkv, int max_ctx) {
   if (B <= 0 || Hkv <= 0 || H <= 0) return 1;
   const long long rows = static_cast<long long>(B) * Hkv * ((H / Hkv + 15) / 16);
-  const long long most = (static_cast<long long>(max_ctx) + 255) / 256, fill = 2ll * rbh::sm_count() / rows;
+  const bool memory = max_ctx > rb::kSdCluster * 1536;
+  const long long each = memory ? 512 : 64, most = (max_ctx + each - 1) / each, fill = 2ll * rbh::sm_count() / rows;
   long long s = fill < most ? fill : most;
   if (s < 1) s = 1;
   if (s > 64) s = 64;
-  if (s < 2 * rb::kSdCluster) {
-    while (s & (s - 1)) s &= s - 1;            // clusters of 2, 4, 8
+  if (!memory || s < 2 * rb::kSdCluster) {
     if (s > rb::kSdCluster) s = rb::kSdCluster;
+    while (s & (s - 1)) s &= s - 1;            // clusters of 2, 4, 8
   }
   return static_cast<int>(s);
 }

@@ -89,14 +89,14 @@ def test_sizes_and_pages(D, dtype, page):
 
 
 # every way of cutting: one part, clusters of 2, 4 and 8, more parts than a cluster; contexts shorter than the longest leave parts empty
-@pytest.mark.parametrize("B,Hkv,ctx", [(150, 2, 600), (64, 2, 700), (30, 2, 1500), (16, 2, 4000), (2, 2, 6000), (1, 1, 40000)])
+@pytest.mark.parametrize("B,Hkv,ctx", [(150, 2, 600), (64, 2, 700), (30, 2, 1500), (16, 2, 4000), (2, 2, 6000), (2, 2, 13000), (1, 1, 40000)])
 @pytest.mark.parametrize("cap", [0.0, 30.0])
 def test_parts(B, Hkv, ctx, cap):
     from rumus_b200.ops import native
     lens = [ctx] + [max(0, ctx - 37 * b * b) for b in range(1, B)]
     args = _case(lens, 4 * Hkv, Hkv, 64, 64, BF, spread=2.0)
     splits = native.lib().rb_span_decode_splits(B, 4 * Hkv, Hkv, ctx)
-    assert splits == {150: 1, 64: 2, 30: 4, 16: 8, 2: 24, 1: 64}[B]
+    assert splits == {600: 1, 700: 2, 1500: 4, 4000: 8, 6000: 8, 13000: 26, 40000: 64}[ctx]
     _check(args, 4 * Hkv, cap=cap)
     _check(args, 4 * Hkv, cap=cap, max_ctx=1)          # a wrong bound on the contexts costs time, not results
 
