@@ -346,8 +346,9 @@ def span_attention(q, k, v, spans=None, causal: bool = True, scale: Optional[flo
 
     ``spans``: int32 ``[B, Sq, 2]`` (or ``[Sq, 2]`` for all batches), row i sees the keys ``lo <= j < hi``; parts outside the keys count as cut off, and
     a row with ``hi <= lo`` gives zeros.  ``causal``: besides, no key behind place ``i + Sk - Sq``.  ``cap``: scores s become cap tanh(s / cap), 0: they
-    stay.  ``slopes``: float32 ``[H]``, what a score loses per place of distance (constants).  Keys and values have to be finite, unseen ones too: a
-    weight of zero times what is not finite is not a number.  On a GPU: bfloat16 or float16 with D a multiple of 8 up to 128, float32 with D up to 128 (a kernel
+    stay.  ``slopes``: float32 ``[H]``, what a score loses per place of distance (constants).  Scores are 32-bit numbers: where even a row's nearest key
+    loses b to the distance, weights (in the gradients) are good to 2^-22 b.  Keys and values have to be finite, unseen ones too: a weight of zero times
+    what is not finite is not a number.  On a GPU: bfloat16 or float16 with D a multiple of 8 up to 128, float32 with D up to 128 (a kernel
     for small models: rows are serial there)."""
     scale = float(scale) if scale is not None else 1.0 / math.sqrt(q.shape[-1])
     cap = float(cap)
