@@ -181,7 +181,7 @@ class MultiheadAttention(Module):
         self.causal = causal
         self.rope_theta = rope_theta
         self.attn_cap, self.alibi = attn_cap, alibi
-        self._slopes = None
+        self._slopes = F.distance_slopes(num_heads, device) if alibi else None
         bound = math.sqrt(1.0 / d_model)
         kv_dim = self.num_kv_heads * self.head_dim
         wq = _uniform((d_model, d_model), bound, _linear_rng, device, dtype)
@@ -202,7 +202,7 @@ class MultiheadAttention(Module):
 
     def slopes(self, device) -> Optional[torch.Tensor]:
         """The heads' slopes on ``device`` (constants, no part of the state), None without ``alibi``."""
-        if self.alibi and (self._slopes is None or self._slopes.device != device):
+        if self.alibi and self._slopes.device != device:
             self._slopes = F.distance_slopes(self.num_heads, device)
         return self._slopes if self.alibi else None
 

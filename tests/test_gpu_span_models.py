@@ -107,3 +107,23 @@ def test_fsdp_step_of_a_packed_model():
     after = model.state_dict()
     assert torch.isfinite(loss) and all(torch.isfinite(v.float()).all() for v in after.values()) and native.read_status() == 0
     assert all(not torch.equal(before[k], after[k]) for k in before if k.endswith("proj.weight"))
+
+
+def test_forward_is_captured_first_and_replayed():
+    """Nothing of a biased layer is made in its first call: that one can be a captured one."""
+    from rumus_b200 import nn
+    from rumus_b200.ops import functional as F
+    m = nn.MultiheadAttention(128, 2, device="cuda", dtype=torch.bfloat16, attn_cap=5.0, alibi=True)
+    other = nn.MultiheadAttention(128, 2, device="cuda", dtype=torch.bfloat16, attn_cap=5.0, alibi=True)
+    x = torch.randn(2, 100, 128, device="cuda").bfloat16()
+    spans = F.document_spans(torch.zeros(2, 100, dtype=torch.int64, device="cuda"))
+    with torch.no_grad():
+        other(x, spans=spans)                       # libraries and kernels are loaded
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = m(x, spans=spans)
+        for _ in range(2):
+            x.copy_(torch.randn(2, 100, 128, device="cuda").bfloat16())
+            graph.replay()
+            assert torch.equal(y, m(x, spans=spans))
