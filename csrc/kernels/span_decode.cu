@@ -392,7 +392,8 @@ int rb_span_decode_splits(int B, int H, int Hkv, int max_ctx) {
 }
 
 // q [B, H, D] with strides q_sb, q_sh in elements, rows 4-byte aligned; caches contiguous, 16-byte aligned, of `pages` pages of `page` tokens; tables [B, max_blocks];
-// ctx, starts (or null) [B]; D a multiple of 8, at most 128.  splits > 8: part_o [splits, B, H, D] and part_lse2 [splits, B, H] are scratch.
+// ctx, starts (or null) [B]; D a multiple of 8, at most 128; out [B, H, D] contiguous, 8-byte aligned.  splits > 8: part_o [splits, B, H, D], 16-byte
+// aligned, and part_lse2 [splits, B, H] are scratch.
 int rb_span_decode(int dtype, int head_major, const void* q, long long q_sb, long long q_sh, const void* k, const void* v, const int* tables, const int* ctx,
                    const int* starts, const float* slopes, void* out, float* part_o, float* part_lse2, int B, int H, int Hkv, int D, int page, int pages,
                    int max_blocks, int splits, float scale, float cap, void* stream) {
@@ -400,6 +401,8 @@ int rb_span_decode(int dtype, int head_major, const void* q, long long q_sb, lon
   if (B <= 0 || H <= 0) return 0;
   if (Hkv <= 0 || H % Hkv || D <= 0 || D > 128 || D % 8 || page <= 0 || pages < 0 || max_blocks < 0 || splits < 1) return 20;
   if (splits > kSdCluster ? !part_o || !part_lse2 : (splits & (splits - 1)) != 0) return 20;
+  const auto off = [](const void* at, uintptr_t bytes) { return reinterpret_cast<uintptr_t>(at) % bytes != 0; };
+  if (off(out, 8) || off(q, 4) || off(k, 16) || off(v, 16) || off(part_o, 16)) return 20;
   SpanDecodeParams p{};
   p.q = q; p.q_sb = q_sb; p.q_sh = q_sh; p.k = k; p.v = v; p.tables = tables; p.ctx = ctx; p.starts = starts;
   p.out = out; p.part_o = part_o; p.part_lse2 = part_lse2;

@@ -30,12 +30,14 @@ __global__ void __launch_bounds__(256)
     f[4] = fmaf(w, y.x, f[4]); f[5] = fmaf(w, y.y, f[5]); f[6] = fmaf(w, y.z, f[6]); f[7] = fmaf(w, y.w, f[7]);
   }
   const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-  *reinterpret_cast<uint4*>(o + r * D + c) =
-      make_uint4(pack2<T>(f[0] * inv, f[1] * inv), pack2<T>(f[2] * inv, f[3] * inv), pack2<T>(f[4] * inv, f[5] * inv), pack2<T>(f[6] * inv, f[7] * inv));
+  // two stores of 8 bytes: decoding's results may begin at any such boundary
+  uint2* to = reinterpret_cast<uint2*>(o + r * D + c);
+  to[0] = make_uint2(pack2<T>(f[0] * inv, f[1] * inv), pack2<T>(f[2] * inv, f[3] * inv));
+  to[1] = make_uint2(pack2<T>(f[4] * inv, f[5] * inv), pack2<T>(f[6] * inv, f[7] * inv));
   if (c == 0 && lse2 != nullptr) lse2[at] = sum == 0.f ? -INFINITY : top + log2f(sum);
 }
 
-// part_o [splits, B, Sq, H, D], part_lse2 [splits, B, H, Sq] -> o [B, Sq, H, D], lse2 [B, H, Sq] (or null)
+// part_o [splits, B, Sq, H, D], 16-byte aligned, part_lse2 [splits, B, H, Sq] -> o [B, Sq, H, D], 8-byte aligned, lse2 [B, H, Sq] (or null)
 template <typename T>
 int launch_span_join(const float* part_o, const float* part_lse2, T* o, float* lse2, int B, int H, int Sq, int D, int splits, cudaStream_t st) {
   const long long pieces = static_cast<long long>(B) * Sq * H * (D / 8), blocks = (pieces + 255) / 256;

@@ -373,7 +373,7 @@ def span_decode(q, k_cache, v_cache, block_tables, ctx_lens, max_ctx: int, scale
     Caches ``[pages, page, Hkv, D]``, with ``head_major`` ``[pages, Hkv, page, D]``; ``block_tables`` int32 ``[B, n]``; ``ctx_lens``, ``starts`` (None:
     0) int32 ``[B]``; ``max_ctx``: no context is longer (decides how contexts are cut; longer ones are still right).  Tokens in pages that the cache
     does not have, and behind the table's end, count as unseen; what pages hold behind a context is never read.  ``cap``, ``slopes``: as in
-    ``span_attention``.  ``out``: contiguous tensor to write into, apart from the others.  On a GPU: bfloat16 or float16, D a multiple of 8 up to
+    ``span_attention``.  ``out``: contiguous tensor to write into, 8-byte aligned, apart from the others.  On a GPU: bfloat16 or float16, D a multiple of 8 up to
     128."""
     if q.dim() != 3 or k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
         raise ValueError(f"decoding of {tuple(q.shape)} over pages {tuple(k_cache.shape)}, {tuple(v_cache.shape)}")
@@ -397,7 +397,8 @@ def span_decode(q, k_cache, v_cache, block_tables, ctx_lens, max_ctx: int, scale
     if out is None:
         out = q.new_empty((B, H, D))
     elif not out.is_contiguous() or out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or out.data_ptr() % 8:
-        raise ValueError(f"decoding writes contiguous heads {tuple(q.shape)} of {q.dtype}, not {out.dtype} {tuple(out.shape)}")
+        raise ValueError(f"decoding writes contiguous heads {tuple(q.shape)} of {q.dtype} on {q.device}, 8-byte aligned, not {out.dtype} {tuple(out.shape)} on "
+                         f"{out.device}")
     elif any(_overlap(out, t) for t in (q, k_cache, v_cache)):
         raise ValueError("decoding reads its queries and pages while it writes: ``out`` has to be apart from them")
     if not q.is_cuda:
