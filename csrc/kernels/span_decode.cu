@@ -72,13 +72,26 @@ __device__ __forceinline__ void span_store4(T* to, float4 v) {
   *reinterpret_cast<uint2*>(to) = make_uint2(pack2<T>(v.x, v.y), pack2<T>(v.z, v.w));
 }
 
-// Eight products -> scores in log2 units.  Few of them and memory to wait for: the tanh in its general form.
+// Eight products -> scores in log2 units.  Whole warp: as in span_score32 a vote decides between the two forms of the tanh (the general one's error grows
+// with the cap, not with the scores).
 template <bool CAP>
 __device__ __forceinline__ void span_scale8(uint32_t* x, const SpanScores& c) {
+  if constexpr (!CAP) {
+    const uint64_t k = both(c.scale2);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float s = __uint_as_float(x[e]);
-    x[e] = __float_as_uint(CAP ? c.out2 - __fdividef(2.f * c.out2, 1.f + fast_exp2(s * (2.f * kLog2e * c.in))) : s * c.scale2);
+    for (int e = 0; e < 8; e += 2) set_pair(x, e, mul_f32x2(pair_at(x, e), k));
+  } else {
+    float reach = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) reach = fmaxf(reach, fabsf(__uint_as_float(x[e])));
+    if (__all_sync(0xffffffffu, reach <= c.near)) {
+      const SpanTanh f(c, c.out2);
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) set_pair(x, e, mul_f32x2(pair_at(x, e), f.r(pair_at(x, e))));
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) set_pair(x, e, mul_f32x2(span_tanh_any(x[e], x[e + 1], c), both(c.out2)));
+    }
   }
 }
 
