@@ -33,6 +33,7 @@ native.register_signature("rb_span_decode", [I, I, P, LL, LL] + [P] * 9 + [I] * 
 
 CLUSTER = 8             # parts of a context that one launch joins (kSdCluster)
 HALVES = (torch.bfloat16, torch.float16)
+_LOG2E = math.log2(math.e)
 
 
 # ---------------------------------------------------------------- spans and slopes
@@ -72,11 +73,23 @@ def distance_slopes(heads: int, device=None) -> torch.Tensor:
 
 
 # ---------------------------------------------------------------- arguments
+def _f32(x: float) -> float:
+    """The nearest 32-bit number, which is what the kernels get."""
+    return c_float(x).value
+
+
+def check_cap(cap: float) -> None:
+    """Refuses caps that 32 bits do not hold, in units of log 2 as the kernels have them: what becomes infinite, or zero, which means none."""
+    if not (cap >= 0.0 and math.isfinite(_f32(cap * _LOG2E)) and (cap == 0.0 or _f32(cap) > 0.0)):
+        raise ValueError(f"a cap is a number of 32 bits above zero, or zero for none, not {cap}")
+
+
 def _scores_ok(heads: int, device, scale: float, cap: float, slopes) -> None:
-    if not math.isfinite(scale):
-        raise ValueError(f"scale {scale}")
-    if not (math.isfinite(cap) and cap >= 0.0):
-        raise ValueError(f"a cap is a number above zero, or zero for none, not {cap}")
+    if not math.isfinite(_f32(scale * _LOG2E)):
+        raise ValueError(f"a scale is a number of 32 bits, not {scale}")
+    check_cap(cap)
+    if cap > 0.0 and not math.isfinite(_f32(2.0 * _LOG2E * scale / cap)):           # the tanh's argument of a product of one
+        raise ValueError(f"a cap of {cap} is too small for a scale of {scale}")
     if slopes is not None:
         if slopes.dtype != torch.float32 or tuple(slopes.shape) != (heads,) or slopes.device != device:
             raise ValueError(f"slopes are float32 [{heads}] on {device}, not {slopes.dtype} {tuple(slopes.shape)} on {slopes.device}")
@@ -346,10 +359,10 @@ def span_attention(q, k, v, spans=None, causal: bool = True, scale: Optional[flo
 
     ``spans``: int32 ``[B, Sq, 2]`` (or ``[Sq, 2]`` for all batches), row i sees the keys ``lo <= j < hi``; parts outside the keys count as cut off, and
     a row with ``hi <= lo`` gives zeros.  ``causal``: besides, no key behind place ``i + Sk - Sq``.  ``cap``: scores s become cap tanh(s / cap), 0: they
-    stay.  ``slopes``: float32 ``[H]``, what a score loses per place of distance (constants).  Scores are 32-bit numbers: where even a row's nearest key
-    loses b to the distance, weights (in the gradients) are good to 2^-22 b.  Keys and values have to be finite, unseen ones too: a weight of zero times
-    what is not finite is not a number.  On a GPU: bfloat16 or float16 with D a multiple of 8 up to 128, float32 with D up to 128 (a kernel
-    for small models: rows are serial there)."""
+    stay.  ``slopes``: float32 ``[H]``, what a score loses per place of distance (constants).  Scores, scale and cap are 32-bit numbers (a scale or a
+    cap that is none is refused): where even a row's nearest key loses b to the distance, weights (in the gradients) are good to 2^-22 b.  Keys and values
+    have to be finite, unseen ones too: a weight of zero times what is not finite is not a number.  On a GPU: bfloat16 or float16 with D a multiple of 8
+    up to 128, float32 with D up to 128 (a kernel for small models: rows are serial there)."""
     scale = float(scale) if scale is not None else 1.0 / math.sqrt(q.shape[-1])
     cap = float(cap)
     _rows_ok(q, k, v, spans, scale, cap, slopes)

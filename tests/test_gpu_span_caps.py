@@ -52,3 +52,12 @@ def test_32_bits(cap):
     want, bound = span_oracle(q, k, v, dout=do, cap=cap)
     for n in got:       # the bound of the 32-bit kernels' other tests
         assert (got[n].double() - want[n]).norm() <= 2e-5 * want[n].norm() + 2 ** -20 * bound[n].norm() / SLACK, n
+
+
+# all scores are plus or minus a cap that is next to nothing: every key weighs the same, and nothing reaches the queries
+@pytest.mark.parametrize("cap", [1e-30, 1e-37])
+def test_caps_far_below_the_scores(cap):
+    q, k, v, do = _inputs(1, 100, 130, 2, 2, 64, BF)
+    got = _check(q, k, v, do, cap=cap)
+    assert (got["dq"] == 0).all() and (got["dk"] == 0).all()
+    _check_decode(_case([300, 1, 5000], 4, 2, 64, 64, BF), 4, cap=cap)
