@@ -98,9 +98,11 @@ class Int4LlamaShard:
         hd = m.d_model // m.num_heads
         self.hd = hd
         self.h_local, self.hkv_local = m.num_heads // world, m.num_kv_heads // world
+        self.shaped = m.attn_cap > 0 or m.alibi       # scores are capped or fall with the distance
+        if self.shaped and torch.device(device).type == "cuda" and not span.kernels_take(cfg.dtype, hd):
+            raise TypeError(f"serving with attn_cap or alibi on a GPU takes bfloat16 or float16 heads of a multiple of 8 numbers up to 128, not {cfg.dtype} of {hd}")
         # this rank's heads' part of the distance bias
         self.slopes = F.distance_slopes(m.num_heads, device)[rank * self.h_local:(rank + 1) * self.h_local].contiguous() if m.alibi else None
-        self.shaped = m.attn_cap > 0 or m.alibi       # scores are capped or fall with the distance
         # row-parallel K splits must fall on quantisation-group boundaries: the FFN width is padded with
         # zero columns (gate, up) / zero rows (down) to a multiple of world x group size, which leaves the
         # function unchanged (silu(0) * 0 = 0 meets zero rows).  Llama-7B: 11008 -> 11264 at 4 and 8 ranks.
