@@ -18,6 +18,7 @@ import torch.nn as nn
 
 from ..nn import Embedding, Module, RMSNorm
 from ..ops import functional as F
+from ..ops.span import check_cap
 from ..parallel.tp import (ColumnParallelLinear, RowParallelLinear, TPContext, gather_rows,
                            mark_tp_replicated, scatter_rows)
 from .llama import LlamaConfig
@@ -31,6 +32,7 @@ class ParallelLlamaBlock(Module):
         self.hd = cfg.d_model // cfg.num_heads
         self.h_local = cfg.num_heads // T
         self.hkv_local = cfg.num_kv_heads // T
+        check_cap(cfg.attn_cap)
         # this rank's heads' part of the distance bias
         self.slopes = F.distance_slopes(cfg.num_heads, device)[tp.rank * self.h_local:(tp.rank + 1) * self.h_local] if cfg.alibi else None
         qkv_out = (cfg.num_heads + 2 * cfg.num_kv_heads) * self.hd

@@ -19,6 +19,7 @@ import torch.nn as nn
 
 from ..ops import functional as F
 from ..ops.attention import f32_covered
+from ..ops.span import check_cap
 
 
 class Module(nn.Module):
@@ -180,6 +181,7 @@ class MultiheadAttention(Module):
         self.head_dim = d_model // num_heads
         self.causal = causal
         self.rope_theta = rope_theta
+        check_cap(attn_cap)
         self.attn_cap, self.alibi = attn_cap, alibi
         self._slopes = F.distance_slopes(num_heads, device) if alibi else None
         bound = math.sqrt(1.0 / d_model)
