@@ -366,7 +366,7 @@ def span_attention(q, k, v, spans=None, causal: bool = True, scale: Optional[flo
     cap that is none is refused): where even a row's nearest key loses b to the distance, weights (in the gradients) are good to 2^-22 b.  Keys and values
     have to be finite, unseen ones too: a weight of zero times what is not finite is not a number.  On a GPU: bfloat16 or float16 with D a multiple of 8
     up to 128, float32 with D up to 128 (a kernel for small models: rows are serial there)."""
-    scale = float(scale) if scale is not None else 1.0 / math.sqrt(q.shape[-1])
+    scale = float(scale) if scale is not None else 1.0 / math.sqrt(q.shape[3]) if q.dim() == 4 and q.shape[3] else 1.0      # else _rows_ok refuses
     cap = float(cap)
     _rows_ok(q, k, v, spans, scale, cap, slopes)
     if not q.is_cuda:

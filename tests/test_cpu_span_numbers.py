@@ -27,3 +27,10 @@ def test_refused(kw):
 def test_taken(kw):
     for call in _calls(**kw):
         assert torch.isfinite(call()).all()
+
+
+@pytest.mark.parametrize("shape", [(1, 3, 2, 0), (), (3, 2, 8)])
+def test_heads_of_nothing_and_other_shapes_are_refused(shape):
+    q = torch.zeros(shape)
+    with pytest.raises(ValueError, match="span attention of"):
+        F.span_attention(q, q, q)
