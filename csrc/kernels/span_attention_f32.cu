@@ -2,9 +2,10 @@
 // each row.  For models that train in 32 bits, whose heads are small: a row is a serial chain over its keys, on the FP32 pipes.  Tiles of 32 rows pass through
 // shared memory; tiles that no row of the CTA reaches are left out.  The backward pass recomputes the weights from the log-sum-exp; its two
 // halves, dQ by query rows and dK, dV by key rows (over all query heads that share the key head), run side by side in one grid, and nothing is added
-// up in memory.  Bound by the FP32 pipes' issue: capped causal heads, forward / forward and backward, against the plain operators with all
-// scores in memory: B 8, S 256, 4 heads of 32: 67 / 178 us (151 / 567); B 4, S 1024, 12 of 64: 0.70 / 2.5 ms (0.92 / 2.2), 9.3 TFLOP/s; B 2, S 2048,
-// 8 of 128: 1.8 / 7.0 ms (1.5 / 3.7).  Larger models belong in 16 bits, where the tensor cores do it.
+// up in memory.  Bound by the FP32 pipes' issue, 9.3 TFLOP/s, or by the chain of a row.  Capped causal heads, us forward / forward and backward, in brackets
+// the plain operators with all scores in memory: B 1, S 256, 4 heads of 32: 64 / 163 (125 / 403); B 4, S 1024, 8 of 64: 501 / 1815 (508 / 1134); B 2, S 2048,
+// 8 of 128: 1843 / 6986 (1297 / 3055).  Calls go to those operators where they are ahead (f32_plain_is_ahead, ops/span.py); rows with spans, and more scores
+// than they should keep, come here.  Larger models belong in 16 bits, where the tensor cores do it.
 #include "attn_f32.cuh"
 #include "span_scores.cuh"
 

@@ -6,8 +6,8 @@
 
 Spans cover packed documents, prompts whose beginning is seen by all of it, windows and padding (``document_spans``).  On a GPU one kernel forward and
 two backward (``csrc/kernels/span_attention_{fwd,bwd}.cu``; in 32 bits one each, ``span_attention_f32.cu``) and one for a new token over pages
-(``span_decode.cu``); on a CPU plain math.  Gradients are
-summed in a fixed order: the same inputs give the same gradients.
+(``span_decode.cu``); long rows in 32 bits go to plain operators where those are faster; on a CPU plain math.  The kernels sum gradients in a fixed order:
+the same inputs give the same gradients.
 """
 from __future__ import annotations
 
@@ -267,26 +267,32 @@ class _SpanAttnFn(torch.autograd.Function):
         return dq, dk, dv, None, None, None, None, None
 
 
+def _span_f32_forward(q, k, v, spans, causal, scale, cap, slopes, lse: bool):
+    """(heads, with ``lse`` the rows' natural log-sum-exp).  Views that the kernels read in place."""
+    B, Sq, H, D = q.shape
+    Sk, Hkv = k.shape[1], k.shape[2]
+    o, lse = _like(q), q.new_empty((B, H, Sq)) if lse else None
+    if q.numel() == 0 or k.numel() == 0:
+        return o.zero_(), lse
+    spans, batch = _spans_arg(spans, Sq)
+    slopes = None if slopes is None else slopes.contiguous()
+    with _on(q.device):
+        at = [_strides(t) for t in (q, k, v)]
+        check(native.lib().rb_span_f32_fwd(D, ptr(q), ptr(k), ptr(v), *map(addressof, at), ptr(spans), batch, ptr(slopes), ptr(o), ptr(lse), B, H, Hkv, Sq, Sk,
+                                           int(causal), scale, cap, stream_ptr()), "rb_span_f32_fwd")
+        count_launch()
+    return o, lse
+
+
 class _SpanF32Fn(torch.autograd.Function):
     """Heads of 16, 32, 64 or 128 numbers in 32 bits."""
 
     @staticmethod
     def forward(ctx, q, k, v, spans, causal, scale, cap, slopes):
         q, k, v = _view(q), _view(k), _view(v)
-        B, Sq, H, D = q.shape
-        Sk, Hkv = k.shape[1], k.shape[2]
-        o, lse = _like(q), q.new_empty((B, H, Sq))
+        o, lse = _span_f32_forward(q, k, v, spans, causal, scale, cap, slopes, True)
         ctx.args = causal, scale, cap
         ctx.save_for_backward(q, k, v, spans, slopes, o, lse)
-        if q.numel() == 0 or k.numel() == 0:
-            return o.zero_()
-        spans, batch = _spans_arg(spans, Sq)
-        slopes = None if slopes is None else slopes.contiguous()
-        with _on(q.device):
-            at = [_strides(t) for t in (q, k, v)]
-            check(native.lib().rb_span_f32_fwd(D, ptr(q), ptr(k), ptr(v), *map(addressof, at), ptr(spans), batch, ptr(slopes), ptr(o), ptr(lse), B, H, Hkv,
-                                               Sq, Sk, int(causal), scale, cap, stream_ptr()), "rb_span_f32_fwd")
-            count_launch()
         return o
 
     @staticmethod
@@ -313,13 +319,77 @@ class _SpanF32Fn(torch.autograd.Function):
         return dq, dk, dv, *none
 
 
-def _span_f32(q, k, v, *args):
+_F32_SIZES = (16, 32, 64, 128)
+
+
+def _span_f32(q, k, v, spans, causal, scale, cap, slopes, grad: bool):
     """Heads of other sizes as the next size that the kernels have, with zeros behind: they add nothing to a product, and come off again."""
     D = q.shape[3]
-    full = next(n for n in (16, 32, 64, 128) if n >= D)
+    full = next(n for n in _F32_SIZES if n >= D)
     if full != D:
         q, k, v = (torch.nn.functional.pad(t, (0, full - D)) for t in (q, k, v))
-    return _SpanF32Fn.apply(q, k, v, *args)[..., :D]
+    if grad:
+        return _SpanF32Fn.apply(q, k, v, spans, causal, scale, cap, slopes)[..., :D]
+    return _span_f32_forward(_view(q), _view(k), _view(v), spans, causal, scale, cap, slopes, False)[0][..., :D]
+
+
+def f32_plain_is_ahead(B: int, H: int, Hkv: int, Sq: int, Sk: int, D: int, causal: bool, grad: bool) -> bool:
+    """Whether the plain operators (``_span_f32_plain``) take less time than the 32-bit kernels, for rows without spans.
+
+    us of a call, estimated by what 500 shapes took (heads of 16 to 128, 4 to 128 batches and heads, 1 to 2048 rows, 128 to 4096 keys, 1 to 8 query heads a
+    key head).  The kernels take their longest chain, 0.27 a key forward and 0.25 + 0.0015 D a key or row more with gradients, or the multiplications at 2.9
+    million a us (0.85 with gradients), whichever is more.  The operators take what the host needs for them, 110 (420), or their passes over the scores.
+    The choice was the faster one or within 1.1 of it for 96 of 100, 1.41 at worst.  Kernels / operators, the rule's in brackets: 2 x 2048 tokens, 8 heads of
+    128: 1843 / [1297], with gradients 6986 / [3055]; 4 x 1024, 8 of 64: [501] / 508 and 1815 / [1134]; a row over 4096 keys, 4 heads of 64:
+    1622 / [79] and 3415 / [336]; 256 tokens, 4 heads of 32: [64] / 125 and [163] / 403; 16 x 256, 8 of 16: [70] / 146 and [183] / 490.
+
+    The operators keep 21 bytes a score: above 2^27 of them (2.8 GB) the kernels serve, which keep none."""
+    rows = min(Sq, Sk) if causal else Sq                                      # that see any key
+    scores = B * H * rows * Sk
+    if scores == 0 or scores > 2 ** 27:
+        return False
+    D = next(n for n in _F32_SIZES if n >= D)
+    work = B * H * D * rows * (Sk - (rows - 1) / 2 if causal else Sk)
+    kernels = max(0.27 * Sk, work / 2.9e6)
+    if not grad:
+        return kernels > max(110.0, scores * (11.0 + 0.065 * D) * 1e-6)
+    kernels += max((0.25 + 0.0015 * D) * max(Sk, rows * H // Hkv), work / 0.85e6)
+    return kernels > max(420.0, scores * (22.0 + 0.18 * D) * 1e-6)
+
+
+def _span_f32_plain(q, k, v, causal: bool, scale: float, cap: float, slopes):
+    """The plain operators for 32-bit heads on a GPU, few passes over the scores: products with the scale (and the cap's reciprocal) in them, tanh, cap,
+    bias and mask at once, softmax, products."""
+    B, Sq, H, D = q.shape
+    Sk, Hkv = k.shape[1], k.shape[2]
+    first = max(Sq - Sk, 0) if causal else 0                                  # rows before it see no key
+    if first:
+        seen = _span_f32_plain(q[:, first:], k, v, causal, scale, cap, slopes)
+        return torch.cat([seen.new_zeros(B, first, H, D), seen], 1)
+    G = H // Hkv
+    qh = q.reshape(B, Sq, Hkv, G, D).permute(0, 2, 3, 1, 4).reshape(B * Hkv, G * Sq, D)
+    kh, vh = (t.transpose(1, 2).reshape(B * Hkv, Sk, D) for t in (k, v))
+    x = torch.baddbmm(q.new_empty(1, 1, 1), qh, kh.transpose(1, 2), beta=0, alpha=scale / cap if cap > 0 else scale)
+    if cap > 0:
+        x = torch.tanh(x) * cap
+    x = x.view(B, H, Sq, Sk)
+    place, key = torch.arange(Sk - Sq, Sk, device=q.device)[:, None], torch.arange(Sk, device=q.device)
+    more = None if slopes is None else -slopes.view(-1, 1, 1) * (place - key).abs()
+    if causal and Sq > 1:
+        more = torch.where(key <= place, 0.0 if more is None else more, -math.inf)
+    if more is not None:
+        x = x + more
+    o = torch.bmm(torch.softmax(x, -1).view(B * Hkv, G * Sq, Sk), vh)
+    return o.view(B, Hkv, G, Sq, D).permute(0, 3, 1, 2, 4).reshape(B, Sq, H, D)
+
+
+def _f32_plain(q, k, spans, causal: bool, scale: float, cap: float, grad: bool) -> bool:
+    """Whether a call in 32 bits goes to the plain operators.  With spans, of which the host knows nothing, the kernels may have far less to do.  The
+    operators have to multiply in 32 bits as the kernels do (no TF32, no automatic rounding to 16 bits), and scale / cap goes into their product: above
+    1e-30, so that no score is below what 32 bits hold."""
+    B, Sq, H, D = q.shape
+    return (spans is None and f32_plain_is_ahead(B, H, k.shape[2], Sq, k.shape[1], D, causal, grad) and (cap == 0.0 or abs(scale) > 1e-30 * cap)
+            and torch.backends.cuda.matmul.fp32_precision in ("none", "ieee") and not torch.is_autocast_enabled("cuda"))
 
 
 # ---------------------------------------------------------------- plain math
@@ -365,18 +435,22 @@ def span_attention(q, k, v, spans=None, causal: bool = True, scale: Optional[flo
     stay.  ``slopes``: float32 ``[H]``, what a score loses per place of distance (constants).  Scores, scale and cap are 32-bit numbers (a scale or a
     cap that is none is refused): where even a row's nearest key loses b to the distance, weights (in the gradients) are good to 2^-22 b.  Keys and values
     have to be finite, unseen ones too: a weight of zero times what is not finite is not a number.  On a GPU: bfloat16 or float16 with D a multiple of 8
-    up to 128, float32 with D up to 128 (a kernel for small models: rows are serial there)."""
+    up to 128, float32 with D up to 128 (a kernel for small models, whose rows are serial; long rows without spans take plain operators, which keep the
+    scores, up to 2^27 of them)."""
     scale = float(scale) if scale is not None else 1.0 / math.sqrt(q.shape[3]) if q.dim() == 4 and q.shape[3] else 1.0      # else _rows_ok refuses
     cap = float(cap)
     _rows_ok(q, k, v, spans, scale, cap, slopes)
     if not q.is_cuda:
         return span_reference(q, k, v, spans, causal, scale, cap, slopes)
+    grad = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
     if q.dtype == torch.float32 and q.shape[3] <= 128:
-        return _span_f32(q, k, v, spans, bool(causal), scale, cap, slopes)
+        if _f32_plain(q, k, spans, bool(causal), scale, cap, grad):
+            return _span_f32_plain(q, k, v, causal, scale, cap, slopes)
+        return _span_f32(q, k, v, spans, bool(causal), scale, cap, slopes, grad)
     if not kernels_take(q.dtype, q.shape[-1]):
         raise TypeError(f"span attention on a GPU takes bfloat16 or float16 heads of a multiple of 8 numbers up to 128, or float32 ones up to 128, not "
                         f"{q.dtype} of {q.shape[-1]}")
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    if grad:
         return _SpanAttnFn.apply(q, k, v, spans, bool(causal), scale, cap, slopes)
     return span_forward(q, k, v, spans, bool(causal), scale, cap, slopes, lse=False, norms=_norms(q, k, cap, slopes))[0]
 

@@ -1,0 +1,61 @@
+"""Span attention in 32 bits where the plain operators are ahead of the kernels: the same bounds against the definition in 64 bits."""
+import pytest
+import torch
+
+from span_oracle import SLACK, span_oracle
+from test_gpu_span import _random_spans, _slopes
+from test_gpu_span_f32 import _check, _run
+
+pytestmark = pytest.mark.gpu
+
+
+# long rows, few rows over many keys, shared key heads, rows before the first key, heads that are no kernel's size
+@pytest.mark.parametrize("B,Sq,Sk,H,Hkv,D", [(1, 1500, 1500, 4, 4, 64), (2, 1, 4096, 4, 2, 32), (1, 64, 3000, 8, 1, 128), (1, 1400, 600, 8, 1, 20),
+                                             (1, 900, 1300, 8, 8, 80)])
+@pytest.mark.parametrize("causal,cap,bias", [(True, 0.0, False), (False, 3.0, False), (True, 3.0, True), (False, 0.0, True)])
+def test_sizes(B, Sq, Sk, H, Hkv, D, causal, cap, bias, monkeypatch):
+    from rumus_b200.ops import span
+    calls = []
+    monkeypatch.setattr(span, "_span_f32_plain", lambda *a, f=span._span_f32_plain: calls.append(a) or f(*a))
+    got = _check(B, Sq, Sk, H, Hkv, D, 2.0, causal=causal, cap=cap, slopes=_slopes(H) if bias else None)
+    assert calls
+    if causal and Sq > Sk:
+        assert (got["o"][:, :Sq - Sk] == 0).all() and (got["dq"][:, :Sq - Sk] == 0).all()
+
+
+def test_views_and_without_gradients():
+    from rumus_b200.ops import functional as F
+    g = torch.Generator(device="cuda").manual_seed(0)
+    x = torch.randn(1, 2048, 3, 4, 64, generator=g, device="cuda")
+    q, k, v = x.unbind(2)
+    do = torch.randn(1, 2048, 1, 64, generator=g, device="cuda").expand(1, 2048, 4, 64)
+    got = _run(q, k, v, do, cap=2.0)
+    want, bound = span_oracle(q, k, v, dout=do, cap=2.0)
+    for n in got:       # as in the kernels' tests
+        assert (got[n].double() - want[n]).norm() <= 2e-5 * want[n].norm() + 2 ** -20 * bound[n].norm() / SLACK, n
+    alone = F.span_attention(q, k, v, cap=2.0)
+    assert (alone.double() - want["o"]).norm() <= 2e-5 * want["o"].norm()
+
+
+def test_the_kernels_serve_what_the_operators_do_not(monkeypatch):
+    """Rows with spans, and products that would be rounded: the kernels' results, in 32 bits."""
+    from rumus_b200.ops import span
+    monkeypatch.setattr(span, "_span_f32_plain", None)
+    _check(1, 1500, 1500, 4, 4, 64, cap=3.0, spans=_random_spans(1, 1500, 1500))
+    monkeypatch.setattr(torch.backends.cuda.matmul, "fp32_precision", "tf32")
+    _check(1, 1500, 1500, 4, 4, 64, cap=3.0)
+
+
+def test_captured_and_replayed():
+    from rumus_b200.ops import functional as F
+    g = torch.Generator(device="cuda").manual_seed(0)
+    q, k, v = (torch.randn(1, 2048, 4, 64, generator=g, device="cuda") for _ in range(3))
+    kw = dict(cap=2.0, slopes=_slopes(4))
+    F.span_attention(q, k, v, **kw)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        o = F.span_attention(q, k, v, **kw)
+    q.copy_(torch.randn(q.shape, generator=g, device="cuda"))
+    graph.replay()
+    assert torch.equal(o, F.span_attention(q, k, v, **kw))
