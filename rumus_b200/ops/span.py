@@ -41,7 +41,7 @@ def document_spans(documents: torch.Tensor, prefix: Optional[torch.Tensor] = Non
     """Spans ``int32 [B, S, 2]`` of packed documents.  ``documents``: ``[B, S]`` whole numbers, equal for neighbouring tokens of one document, negative
     for padding (sees nothing, is seen by none).  A token sees its own document: all of it, with ``causal`` up to itself.  ``prefix``: ``[B, S]``
     truth values; with ``causal`` a document's tokens up to the last of its leading run of them see one another (and all later ones of the document
-    see them)."""
+    see them).  For ``span_attention`` with ``causal=False``: the spans stand in the causal mask's place, which would cut a prefix off."""
     if documents.dim() != 2 or documents.dtype.is_floating_point or documents.dtype == torch.bool:
         raise ValueError(f"documents are whole numbers [B, S], not {documents.dtype} {tuple(documents.shape)}")
     B, S = documents.shape
@@ -172,10 +172,11 @@ def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
 
 # ---------------------------------------------------------------- kernels
 def _norms(q, k, cap: float, slopes):
-    """Room for the lengths of queries and keys, by which biased scores without a cap are known to be too far for a weight; None where it does not pay.
+    """Room for the lengths of queries and keys, by which biased scores without a cap are known to be too far for a weight; None where they are not noted.
     One pass over both is linear in the rows, what it saves grows with their square.  Without / with it, usual slopes: 2 x 4096 rows, 32 heads over 8 of 128:
     forward 312 / 257 us, backward 993 / 844; 8192 rows, 16 heads over 4: 273 / 187 and 940 / 651; 4 x 2048 rows, 16 heads of 64: 100 / 105 and 281 / 247;
-    512 rows over 8192 keys, 32 heads over 8: forward 181 / 193."""
+    512 rows over 8192 keys, 32 heads over 8: forward 181 / 193.  One limit serves calls with and without gradients, where either gains: with gradients
+    2048 rows would gain too (8 % of the two passes), and do without."""
     if slopes is None or cap > 0 or q.shape[1] < 1024 or k.shape[1] < 4096:
         return None
     return torch.empty((q.shape[0], q.shape[2] + k.shape[2], 32), dtype=torch.float32, device=q.device)
@@ -432,11 +433,13 @@ def span_attention(q, k, v, spans=None, causal: bool = True, scale: Optional[flo
 
     ``spans``: int32 ``[B, Sq, 2]`` (or ``[Sq, 2]`` for all batches), row i sees the keys ``lo <= j < hi``; parts outside the keys count as cut off, and
     a row with ``hi <= lo`` gives zeros.  ``causal``: besides, no key behind place ``i + Sk - Sq``.  ``cap``: scores s become cap tanh(s / cap), 0: they
-    stay.  ``slopes``: float32 ``[H]``, what a score loses per place of distance (constants).  Scores, scale and cap are 32-bit numbers (a scale or a
-    cap that is none is refused): where even a row's nearest key loses b to the distance, weights (in the gradients) are good to 2^-22 b.  Keys and values
-    have to be finite, unseen ones too: a weight of zero times what is not finite is not a number.  On a GPU: bfloat16 or float16 with D a multiple of 8
-    up to 128, float32 with D up to 128 (a kernel for small models, whose rows are serial; long rows without spans take plain operators, which keep the
-    scores, up to 2^27 of them)."""
+    stay.  ``slopes``: float32 ``[H]``, what a score loses per place of distance (constants).
+
+    Scores, scale and cap are 32-bit numbers (a scale or a cap that is none is refused): where even a row's nearest key loses b to the distance, weights (in
+    the gradients) are good to 2^-22 b, and under a cap below the rounding of products, 2^-22 of what they are made of, gradients of scores next to zero
+    are arbitrary.  Keys and values have to be finite, unseen ones too: a weight of zero times what is not finite is not a number.  On a GPU: bfloat16 or
+    float16 with D a multiple of 8 up to 128, float32 with D up to 128 (a kernel for small models, whose rows are serial; long rows without spans take
+    plain operators, which keep the scores, up to 2^27 of them)."""
     scale = float(scale) if scale is not None else 1.0 / math.sqrt(q.shape[3]) if q.dim() == 4 and q.shape[3] else 1.0      # else _rows_ok refuses
     cap = float(cap)
     _rows_ok(q, k, v, spans, scale, cap, slopes)
@@ -457,8 +460,8 @@ def span_attention(q, k, v, spans=None, causal: bool = True, scale: Optional[flo
 
 def span_decode(q, k_cache, v_cache, block_tables, ctx_lens, max_ctx: int, scale: Optional[float] = None, cap: float = 0.0, slopes=None, starts=None,
                 head_major: bool = False, out=None):
-    """Span attention of one token per sequence over pages: ``q [B, H, D]`` sees the tokens ``starts[b] <= t < ctx_lens[b]`` of its sequence, itself the
-    last of them; returns ``[B, H, D]`` (zeros where it sees none).
+    """Span attention of one token per sequence over pages (for serving: no gradients on a GPU): ``q [B, H, D]`` sees the tokens
+    ``starts[b] <= t < ctx_lens[b]`` of its sequence, itself the last of them; returns ``[B, H, D]`` (zeros where it sees none).
 
     Caches ``[pages, page, Hkv, D]``, with ``head_major`` ``[pages, Hkv, page, D]``; ``block_tables`` int32 ``[B, n]``; ``ctx_lens``, ``starts`` (None:
     0) int32 ``[B]``; ``max_ctx``: no context is longer (decides how contexts are cut; longer ones are still right).  Tokens in pages that the cache
