@@ -14,13 +14,17 @@ def test_the_rule_follows_its_measurements(shape, forward, grad):
     assert f32_plain_is_ahead(*shape, True, False) == forward and f32_plain_is_ahead(*shape, True, True) == grad
 
 
-def test_never_where_the_scores_are_too_many_or_rounded(monkeypatch):
+def test_never_where_the_scores_are_too_many_or_rounded_or_the_call_is_captured(monkeypatch):
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)       # without a GPU it raises
     q = torch.empty(1, 2048, 8, 128)
     args = (True, 1.0, 0.0, True)
     assert _f32_plain(q, q, None, *args) and not _f32_plain(q, q, torch.zeros(2048, 2, dtype=torch.int32), *args)
     assert not _f32_plain(q, q, None, True, 1.0, 1e31, True) and not f32_plain_is_ahead(8, 32, 32, 2048, 2048, 128, True, True)
     with monkeypatch.context() as m:
         m.setattr(torch, "is_autocast_enabled", lambda kind: kind == "cuda")
+        assert not _f32_plain(q, q, None, *args)
+    with monkeypatch.context() as m:
+        m.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
         assert not _f32_plain(q, q, None, *args)
     was = torch.backends.cuda.matmul.fp32_precision
     try:

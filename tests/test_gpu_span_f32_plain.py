@@ -46,16 +46,48 @@ def test_the_kernels_serve_what_the_operators_do_not(monkeypatch):
     _check(1, 1500, 1500, 4, 4, 64, cap=3.0)
 
 
-def test_captured_and_replayed():
-    from rumus_b200.ops import functional as F
+FIRST = """
+import torch
+from rumus_b200.ops import functional as F, native
+native.lib()
+g = torch.Generator(device="cuda").manual_seed(0)
+leaves = [torch.randn(1, 2048, 4, 64, generator=g, device="cuda").requires_grad_(True) for _ in range(3)]
+do = torch.randn(1, 2048, 4, 64, generator=g, device="cuda")
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    o = F.span_attention(*leaves, cap=2.0)
+    grads = torch.autograd.grad(o, leaves, do)
+with torch.no_grad():
+    leaves[0].mul_(0.5)
+graph.replay()
+now = F.span_attention(*leaves, cap=2.0)
+for a, b in zip((o, *grads), (now, *torch.autograd.grad(now, leaves, do))):
+    assert (a - b).norm() <= 4e-5 * b.norm()          # each within 2e-5 of the definition
+print("replayed")
+"""
+
+
+def test_a_process_may_begin_with_a_captured_call():
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", FIRST], cwd=root, env={**os.environ, "PYTHONPATH": root}, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "replayed" in r.stdout, r.stderr[-2000:]
+
+
+def test_captured_and_replayed(monkeypatch):
+    from rumus_b200.ops import functional as F, span
     g = torch.Generator(device="cuda").manual_seed(0)
     q, k, v = (torch.randn(1, 2048, 4, 64, generator=g, device="cuda") for _ in range(3))
     kw = dict(cap=2.0, slopes=_slopes(4))
     F.span_attention(q, k, v, **kw)
     torch.cuda.synchronize()
+    monkeypatch.setattr(span, "_span_f32_plain", None)          # a captured call takes the kernels
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         o = F.span_attention(q, k, v, **kw)
     q.copy_(torch.randn(q.shape, generator=g, device="cuda"))
     graph.replay()
-    assert torch.equal(o, F.span_attention(q, k, v, **kw))
+    assert torch.equal(o, span._span_f32(q, k, v, None, True, 64 ** -0.5, 2.0, kw["slopes"], False))
