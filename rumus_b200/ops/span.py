@@ -388,11 +388,11 @@ def _f32_plain(q, k, spans, causal: bool, scale: float, cap: float, grad: bool) 
     """Whether a call in 32 bits goes to the plain operators.  With spans, of which the host knows nothing, the kernels may have far less to do.  The
     operators have to multiply in 32 bits as the kernels do (no TF32, no automatic rounding to 16 bits), and scale / cap goes into their product: above
     1e-30, so that no score is below what 32 bits hold.  A call that is captured takes the kernels: the library of the products cannot be
-    loaded then, and a thread's first call may be one."""
+    loaded then, and a thread's first call may be one.  So does one under torch's deterministic algorithms, which refuse those products."""
     B, Sq, H, D = q.shape
     return (spans is None and f32_plain_is_ahead(B, H, k.shape[2], Sq, k.shape[1], D, causal, grad) and (cap == 0.0 or abs(scale) > 1e-30 * cap)
             and torch.backends.cuda.matmul.fp32_precision in ("none", "ieee") and not torch.is_autocast_enabled("cuda")
-            and not torch.cuda.is_current_stream_capturing())
+            and not torch.are_deterministic_algorithms_enabled() and not torch.cuda.is_current_stream_capturing())
 
 
 # ---------------------------------------------------------------- plain math

@@ -47,3 +47,16 @@ def test_the_operators_compute_what_the_reference_does(Sq, Sk, H, Hkv, D, causal
         assert (a[:, :Sq - Sk] == 0).all()
     for x, y in zip(torch.autograd.grad(a, (q, k, v), do), torch.autograd.grad(b, (q, k, v), do)):
         assert torch.allclose(x, y, atol=1e-12)
+
+
+def test_never_under_deterministic_algorithms(monkeypatch):
+    """They refuse the library's products, unless a variable of the environment is set; the kernels need none."""
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    q = torch.empty(1, 2048, 8, 128)
+    was = torch.are_deterministic_algorithms_enabled()
+    try:
+        torch.use_deterministic_algorithms(True)
+        assert not _f32_plain(q, q, None, True, 1.0, 0.0, True)
+    finally:
+        torch.use_deterministic_algorithms(was)
+    assert _f32_plain(q, q, None, True, 1.0, 0.0, True)

@@ -77,6 +77,17 @@ def test_a_process_may_begin_with_a_captured_call():
     assert r.returncode == 0 and "replayed" in r.stdout, r.stderr[-2000:]
 
 
+def test_deterministic_algorithms():
+    """The kernels serve, whose results two runs share."""
+    was = torch.are_deterministic_algorithms_enabled()
+    try:
+        torch.use_deterministic_algorithms(True)
+        a, b = (_check(1, 1500, 1500, 4, 4, 64, cap=3.0) for _ in range(2))
+    finally:
+        torch.use_deterministic_algorithms(was)
+    assert all(torch.equal(a[n], b[n]) for n in a)
+
+
 def test_captured_and_replayed(monkeypatch):
     from rumus_b200.ops import functional as F, span
     g = torch.Generator(device="cuda").manual_seed(0)
