@@ -3,8 +3,8 @@
 // shared memory; tiles that no row of the CTA reaches are left out.  The backward pass recomputes the weights from the log-sum-exp; its two
 // halves, dQ by query rows and dK, dV by key rows (over all query heads that share the key head), run side by side in one grid, and nothing is added
 // up in memory.  Bound by the FP32 pipes' issue, 9.3 TFLOP/s, or by the chain of a row.  Capped causal heads, us forward / forward and backward, in brackets
-// the plain operators with all scores in memory: B 1, S 256, 4 heads of 32: 64 / 163 (125 / 403); B 4, S 1024, 8 of 64: 501 / 1815 (508 / 1134); B 2, S 2048,
-// 8 of 128: 1843 / 6986 (1297 / 3055).  Calls go to those operators where they are ahead (f32_plain_is_ahead, ops/span.py); rows with spans, and more scores
+// the plain operators with all scores in memory: B 1, S 256, 4 heads of 32: 64 / 163 (105 / 428); B 4, S 1024, 8 of 64: 501 / 1826 (543 / 1310); B 2, S 2048,
+// 8 of 128: 1814 / 6977 (1368 / 3399).  Calls go to those operators where they are ahead (f32_plain_is_ahead, ops/span.py); rows with spans, and more scores
 // than they should keep, come here.  Larger models belong in 16 bits, where the tensor cores do it.
 #include "attn_f32.cuh"
 #include "span_scores.cuh"

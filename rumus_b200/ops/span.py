@@ -339,10 +339,10 @@ def f32_plain_is_ahead(B: int, H: int, Hkv: int, Sq: int, Sk: int, D: int, causa
 
     us of a call, estimated by what 500 shapes took (heads of 16 to 128, 4 to 128 batches and heads, 1 to 2048 rows, 128 to 4096 keys, 1 to 8 query heads a
     key head).  The kernels take their longest chain, 0.27 a key forward and 0.25 + 0.0015 D a key or row more with gradients, or the multiplications at 2.9
-    million a us (0.85 with gradients), whichever is more.  The operators take what the host needs for them, 110 (420), or their passes over the scores.
-    The choice was the faster one or within 1.1 of it for 96 of 100, 1.41 at worst.  Kernels / operators, the rule's in brackets: 2 x 2048 tokens, 8 heads of
-    128: 1843 / [1297], with gradients 6986 / [3055]; 4 x 1024, 8 of 64: [501] / 508 and 1815 / [1134]; a row over 4096 keys, 4 heads of 64:
-    1622 / [79] and 3415 / [336]; 256 tokens, 4 heads of 32: [64] / 125 and [163] / 403; 16 x 256, 8 of 16: [70] / 146 and [183] / 490.
+    million a us (0.85 with gradients), whichever is more.  The operators take what the host needs for them, 100 (390), or their passes over the scores.
+    The choice was the faster one or within 1.1 of it for 95 of 100, 1.43 at worst.  Kernels / operators, the rule's in brackets: 2 x 2048 tokens, 8 heads of
+    128: 1814 / [1368], with gradients 6977 / [3399]; 4 x 1024, 8 of 64: [501] / 543 and 1826 / [1310]; a row over 4096 keys, 4 heads of 64:
+    1622 / [76] and 3418 / [310]; 256 tokens, 4 heads of 32: [64] / 105 and [163] / 428; 16 x 256, 8 of 16: [70] / 130 and [183] / 476.
 
     The operators keep 21 bytes a score: above 2^27 of them (2.8 GB) the kernels serve, which keep none."""
     rows = min(Sq, Sk) if causal else Sq                                      # that see any key
@@ -353,14 +353,14 @@ def f32_plain_is_ahead(B: int, H: int, Hkv: int, Sq: int, Sk: int, D: int, causa
     work = B * H * D * rows * (Sk - (rows - 1) / 2 if causal else Sk)
     kernels = max(0.27 * Sk, work / 2.9e6)
     if not grad:
-        return kernels > max(110.0, scores * (11.0 + 0.065 * D) * 1e-6)
+        return kernels > max(100.0, scores * (12.0 + 0.067 * D) * 1e-6)
     kernels += max((0.25 + 0.0015 * D) * max(Sk, rows * H // Hkv), work / 0.85e6)
-    return kernels > max(420.0, scores * (22.0 + 0.18 * D) * 1e-6)
+    return kernels > max(390.0, scores * (26.0 + 0.19 * D) * 1e-6)
 
 
 def _span_f32_plain(q, k, v, causal: bool, scale: float, cap: float, slopes):
     """The plain operators for 32-bit heads on a GPU, few passes over the scores: products with the scale (and the cap's reciprocal) in them, tanh, cap,
-    bias and mask at once, softmax, products."""
+    bias, mask, softmax, products."""
     B, Sq, H, D = q.shape
     Sk, Hkv = k.shape[1], k.shape[2]
     first = max(Sq - Sk, 0) if causal else 0                                  # rows before it see no key
@@ -375,11 +375,10 @@ def _span_f32_plain(q, k, v, causal: bool, scale: float, cap: float, slopes):
         x = torch.tanh(x) * cap
     x = x.view(B, H, Sq, Sk)
     place, key = torch.arange(Sk - Sq, Sk, device=q.device)[:, None], torch.arange(Sk, device=q.device)
-    more = None if slopes is None else -slopes.view(-1, 1, 1) * (place - key).abs()
+    if slopes is not None:
+        x = x - slopes.view(-1, 1, 1) * (place - key).abs()
     if causal and Sq > 1:
-        more = torch.where(key <= place, 0.0 if more is None else more, -math.inf)
-    if more is not None:
-        x = x + more
+        x = x.masked_fill(key > place, -math.inf)                             # not added: what unseen keys' products are, infinite too, decides nothing
     o = torch.bmm(torch.softmax(x, -1).view(B * Hkv, G * Sq, Sk), vh)
     return o.view(B, Hkv, G, Sq, D).permute(0, 3, 1, 2, 4).reshape(B, Sq, H, D)
 

@@ -37,6 +37,19 @@ def test_views_and_without_gradients():
     assert (alone.double() - want["o"]).norm() <= 2e-5 * want["o"].norm()
 
 
+@pytest.mark.parametrize("cap,bias", [(0.0, False), (3.0, True)])
+def test_unseen_keys_of_any_size_decide_nothing(cap, bias):
+    """Rows before keys whose products leave 32 bits' range: as if these were ordinary numbers."""
+    from rumus_b200.ops import functional as F
+    g = torch.Generator(device="cuda").manual_seed(0)
+    q, k, v = (torch.randn(1, 2048, 4, 64, generator=g, device="cuda") for _ in range(3))
+    kw = dict(cap=cap, slopes=_slopes(4) if bias else None)
+    want = F.span_attention(q, k, v, **kw)
+    big = torch.finfo(torch.float32).max
+    k[:, 2000:], v[:, 2000:] = big / 8 * k[:, 2000:].sign(), big / 8
+    assert torch.equal(F.span_attention(q, k, v, **kw)[:, :2000], want[:, :2000])
+
+
 def test_the_kernels_serve_what_the_operators_do_not(monkeypatch):
     """Rows with spans, and products that would be rounded: the kernels' results, in 32 bits."""
     from rumus_b200.ops import span
