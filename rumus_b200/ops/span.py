@@ -114,9 +114,14 @@ def _rows_ok(q, k, v, spans, scale, cap, slopes) -> None:
     _scores_ok(H, q.device, scale, cap, slopes)
 
 
-def kernels_take(dtype: torch.dtype, D: int) -> bool:
+def kernels_cover(dtype: torch.dtype, D: int) -> bool:
     """Whether the 16-bit GPU kernels cover heads of this type and size."""
     return dtype in HALVES and D % 8 == 0 and 0 < D <= 128
+
+
+def kernels_take(q: torch.Tensor) -> bool:
+    """Whether the 16-bit GPU kernels cover heads of this tensor's type and size."""
+    return kernels_cover(q.dtype, q.shape[-1])
 
 
 _HERE = nullcontext()
@@ -185,7 +190,7 @@ def _norms(q, k, cap: float, slopes):
 def span_forward(q, k, v, spans, causal: bool, scale: float, cap: float, slopes, out=None, lse: bool = True, norms=None):
     """Heads ``[B, Sq, H, D]`` and, with ``lse``, the rows' log-sum-exp in units of log 2 ``[B, H, Sq]``.  For heads that ``kernels_take``.  ``out``:
     contiguous tensor to write into; ``norms``: from ``_norms``."""
-    if not kernels_take(q.dtype, q.shape[3]) or not q.dtype == k.dtype == v.dtype:
+    if not kernels_take(q) or not q.dtype == k.dtype == v.dtype:
         raise TypeError(f"span attention's kernels take bfloat16 or float16 heads of a multiple of 8 numbers up to 128, not {q.dtype}, {k.dtype}, {v.dtype} of "
                         f"{q.shape[3]}")
     q, k, v = _view(q), _view(k), _view(v)
@@ -451,7 +456,7 @@ def span_attention(q, k, v, spans=None, causal: bool = True, scale: Optional[flo
         if _f32_plain(q, k, spans, bool(causal), scale, cap, grad):
             return _span_f32_plain(q, k, v, causal, scale, cap, slopes)
         return _span_f32(q, k, v, spans, bool(causal), scale, cap, slopes, grad)
-    if not kernels_take(q.dtype, q.shape[-1]):
+    if not kernels_take(q):
         raise TypeError(f"span attention on a GPU takes bfloat16 or float16 heads of a multiple of 8 numbers up to 128, or float32 ones up to 128, not "
                         f"{q.dtype} of {q.shape[-1]}")
     if grad:
@@ -497,7 +502,7 @@ def span_decode(q, k_cache, v_cache, block_tables, ctx_lens, max_ctx: int, scale
         raise ValueError("decoding reads its queries and pages while it writes: ``out`` has to be apart from them")
     if not q.is_cuda:
         return out.copy_(_decode_reference(q, k_cache, v_cache, block_tables, ctx_lens, scale, cap, slopes, starts, head_major))
-    if not kernels_take(q.dtype, q.shape[-1]):
+    if not kernels_take(q):
         raise TypeError(f"decoding on a GPU takes bfloat16 or float16 heads of a multiple of 8 numbers up to 128, not {q.dtype} of {D}")
     if not k_cache.is_contiguous() or not v_cache.is_contiguous() or k_cache.data_ptr() % 16 or v_cache.data_ptr() % 16:
         raise ValueError("the caches' pages are contiguous and 16-byte aligned")

@@ -100,7 +100,7 @@ class Int4LlamaShard:
         self.h_local, self.hkv_local = m.num_heads // world, m.num_kv_heads // world
         span.check_cap(m.attn_cap)
         self.shaped = m.attn_cap > 0 or m.alibi       # scores are capped or fall with the distance
-        if self.shaped and torch.device(device).type == "cuda" and not span.kernels_take(cfg.dtype, hd):
+        if self.shaped and torch.device(device).type == "cuda" and not span.kernels_cover(cfg.dtype, hd):
             raise TypeError(f"serving with attn_cap or alibi on a GPU takes bfloat16 or float16 heads of a multiple of 8 numbers up to 128, not {cfg.dtype} of {hd}")
         # this rank's heads' part of the distance bias
         self.slopes = F.distance_slopes(m.num_heads, device)[rank * self.h_local:(rank + 1) * self.h_local].contiguous() if m.alibi else None
