@@ -201,9 +201,10 @@ __device__ __forceinline__ int4 span_range_join(int4 a, int4 b) {
 namespace rbh {
 
 // What a call's scale and cap are to the kernels.  tanh(u) = u P(u^2) for |u| <= 0.625, P of degree 3 fitted so that the largest relative error is least:
-// 3.1e-6.  At scores of 30 a weight is then off by 9.3e-5 of itself: a forty-second of bf16's rounding (half a step, 2^-8), a fifth of fp16's.  Of caps far above the scale the highest coefficients in the products are below
-// fp32's range: they are left out, and the polynomial holds as far as they make no more difference than that.  (The general form, whose error is
-// absolute, is no choice there: 3e-7 of a cap of 1e6 is 0.3.)  Of caps far below the scale they are above it, and the general form serves.
+// 3.1e-6.  At scores of 30 a weight is then off by 9.3e-5 of itself: a forty-second of bf16's rounding (half a step, 2^-8), a fifth of fp16's.  Of caps
+// far above the scale the highest coefficients in the products are below fp32's range: they are left out, and the polynomial holds as far as they make no
+// more difference than that.  (The general form, whose error is absolute, is no choice there: 3e-7 of a cap of 1e6 is 0.3.)  Of caps far below the scale
+// they are above it, and the general form serves.
 inline rb::SpanScores span_scores(float scale, float cap) {
   rb::SpanScores c{};
   c.scale2 = scale * rb::kLog2e;
